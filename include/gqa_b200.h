@@ -614,6 +614,239 @@ typedef struct gqa_qkv_params {
 size_t gqa_qkv_workspace_bytes(int32_t hidden, int32_t num_q_heads, int32_t num_kv_heads);
 int gqa_qkv_gemv(const gqa_qkv_params* p);
 
+/* ---- tree-drafted decoding ------------------------------------------------------------------ */
+/*
+ * A decode loop that drafts several tokens per step keeps them as a TREE behind each sequence's
+ * history: node 0 is the root (the newest committed token, whose cache row is written in this step
+ * too), every other node follows its parent in index order (parent < node). One step is
+ *   gqa_rope_append   the nodes' query and key rows rotated to position history + depth, key and
+ *                     value rows appended to the cache slots history + node;
+ *   gqa_tree_decode   attention of all nodes over the history and their own ancestors;
+ *   gqa_tree_verify   the target's probabilities against the draft: accepted path and next token;
+ *   gqa_tree_commit   the accepted path's cache rows moved to slots history, history + 1, ...
+ * The reference has no counterpart: it decodes one token per step (main/main_qwen3.cpp:58-96).
+ *
+ * In all four, seq_lens_dev[b] counts the history AND the nodes (as q_tokens counts its tokens),
+ * and tree_sizes_dev[b] (null: `tokens` for every sequence) is the number of nodes n_b: node t lies
+ * in slot seq_len - n_b + t. n_b may differ from sequence to sequence and may be 0 (nothing to do).
+ * Rows t >= n_b of per-node outputs are left as they were. A sequence whose length or size is out of
+ * range (n_b < 0, n_b > tokens, seq_len < n_b, seq_len beyond what its blocks hold) is skipped and
+ * *status_dev (optional) set to GQA_STATUS_BAD_INPUT. At most GQA_TREE_MAX_TOKENS nodes.
+ */
+#define GQA_TREE_MAX_TOKENS 128
+
+/*
+ * Host only. From parents [batch, tokens] (-1 at node 0, else 0 <= parent < node; entries of nodes
+ * >= sizes[b] are ignored; sizes null: all `tokens`) the mask rows gqa_tree_decode reads
+ * (mask [batch, tokens, (tokens + 31) / 32]: bit j % 32 of word j / 32 of row t is set when node t sees
+ * node j, which is itself and its ancestors) and each node's depth [batch, tokens] (root 0). Either
+ * output may be null. GQA_ERR_RANGE on a parent that breaks the order.
+ */
+int gqa_tree_masks(const int32_t* parents, const int32_t* sizes, int32_t batch, int32_t tokens,
+                   uint32_t* mask, int32_t* depth);
+
+/* Pairing of the rotated channels: (i, i + rotary_dim / 2), or (2 i, 2 i + 1). */
+#define GQA_ROPE_HALF 0
+#define GQA_ROPE_INTERLEAVED 1
+
+/* How the frequencies base^(-2 i / rotary_dim) are stretched for contexts beyond the trained one. */
+#define GQA_ROPE_SCALE_NONE 0
+#define GQA_ROPE_SCALE_LINEAR 1 /* all divided by `factor` (position interpolation) */
+#define GQA_ROPE_SCALE_NTK 2    /* base * factor^(r / (r - 2)), r = rotary_dim > 2 */
+#define GQA_ROPE_SCALE_YARN 3   /* YaRN: pairs that turn less than beta_slow times over original_len
+                                   positions divided by `factor`, those above beta_fast kept, the rest
+                                   interpolated linearly in the number of turns */
+
+/*
+ * Host only: freq[rotary_dim / 2] in radians per position, FP64, and the factor sine and cosine are
+ * multiplied by (1, or 0.1 ln(factor) + 1 for YaRN). base <= 0 means the 1e6 of gqa_sin_cos_cache;
+ * beta_fast / beta_slow <= 0 mean 32 and 1. factor >= 1.
+ */
+int gqa_rope_frequencies(int32_t rotary_dim, double base, int32_t scaling, double factor,
+                         int32_t original_len, double beta_fast, double beta_slow, double* freq,
+                         float* attn_factor);
+
+/*
+ * Rotary positions with the KV append, the general form of gqa_qk_norm_rope_append: any frequencies,
+ * both pairings, part of the head, cache slot and rotary position of a row apart, optional QK-Norm.
+ * Row (b, t) has slot seq_len_b - n_b + t and rotary position seq_len_b - n_b + depth[b, t] (depth_dev
+ * null: t). With theta_i = position * freq[i] and (x_a, x_c) the i-th pair of a head,
+ *     y_a = f (x_a cos theta_i - x_c sin theta_i),  y_c = f (x_a sin theta_i + x_c cos theta_i),
+ * f = attn_factor; channels >= rotary_dim pass unchanged. With qk_weight every query and key head is
+ * first RMS-normalised over its 128 channels (eps) and scaled by qk_weight[0:128] (queries) or
+ * [128:256] (keys). Angles are reduced in FP64 (they stay exact at far positions, unlike the FP32 tables
+ * of gqa_sin_cos_cache), the rest is FP32 with one rounding at the end.
+ *   dtype            GQA_DTYPE_BF16 or GQA_DTYPE_F32: rows, weights and caches.
+ *   q, q_out         [batch, tokens, num_q_heads, 128], *_token_stride elements between tokens (0:
+ *                    packed; sequences follow at tokens * stride). q_out may be q with the same stride.
+ *   k_new, v_new     [batch, tokens, num_kv_heads, 128] likewise. They must not overlap the caches.
+ *   rotary_dim       a multiple of 8, 8 .. 128.
+ * All row pointers and strides are 16-byte aligned.
+ */
+typedef struct gqa_rope_params {
+    int32_t dtype;
+    int32_t batch;
+    int32_t tokens;
+    int32_t num_q_heads;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t rotary_dim;
+    int32_t style;
+    int32_t blocks_per_seq;
+    int32_t fixed_block;
+    float eps;
+    float attn_factor;
+    gqa_kv_layout layout;
+    int64_t q_token_stride;
+    int64_t q_out_token_stride;
+    int64_t k_token_stride;
+    int64_t v_token_stride;
+    const void* q;
+    void* q_out;
+    const void* k_new;
+    const void* v_new;
+    const void* qk_weight;         /* [256], or null: no normalisation */
+    const double* freq_dev;        /* [rotary_dim / 2] on the device */
+    void* k_cache;
+    void* v_cache;
+    const int32_t* seq_lens_dev;   /* [batch] */
+    const int32_t* tree_sizes_dev; /* [batch] or null */
+    const int32_t* depth_dev;      /* [batch, tokens] or null */
+    const int32_t* block_table_dev;
+    int32_t* status_dev;
+    void* stream;
+} gqa_rope_params;
+
+int gqa_rope_append(const gqa_rope_params* p);
+
+/*
+ * Attention of every node over the history and the nodes its mask row names:
+ *     out[b, t, h] = sum_j softmax_j(q[b, t, h] . k[j] / sqrt(128)) v[j],
+ * j over positions < seq_len_b - n_b and over nodes j < n_b with bit j of mask row (b, t) set (any
+ * pattern, not only ancestors). mask_dev null: node t sees nodes 0 .. t (a causal run). A row that
+ * sees nothing gives zeros. Key and value rows that no row of the output sees may hold anything,
+ * infinities and NaN included.
+ *   dtype          GQA_DTYPE_BF16 or GQA_DTYPE_F32 (q, out and caches).
+ *   q, out         [batch, tokens, num_q_heads, 128], q_token_stride elements between tokens of q (0:
+ *                  packed; sequences follow at tokens * stride), out packed. num_q_heads /
+ *                  num_kv_heads <= 8.
+ *   layout, block_table_dev, blocks_per_seq, fixed_block   as in gqa_decode_params; batch <= 1024.
+ *   workspace      gqa_tree_workspace_bytes() bytes, 16-byte aligned, no initialisation; calls that
+ *                  may overlap (streams, concurrent graph launches) need one each.
+ */
+typedef struct gqa_tree_decode_params {
+    int32_t dtype;
+    int32_t batch;
+    int32_t tokens;
+    int32_t num_q_heads;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t blocks_per_seq;
+    int32_t fixed_block;
+    gqa_kv_layout layout;
+    int64_t q_token_stride;
+    const void* q;
+    const void* k_cache;
+    const void* v_cache;
+    void* out;
+    const uint32_t* mask_dev;      /* [batch, tokens, (tokens + 31) / 32] or null */
+    const int32_t* seq_lens_dev;   /* [batch] */
+    const int32_t* tree_sizes_dev; /* [batch] or null */
+    const int32_t* block_table_dev;
+    void* workspace;
+    size_t workspace_bytes;
+    int32_t* status_dev;
+    void* stream;
+} gqa_tree_decode_params;
+
+/* sm_count 0 asks the current device. 0 when the shape is not supported. */
+size_t gqa_tree_workspace_bytes(int32_t dtype, int32_t batch, int32_t tokens, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t sm_count);
+int gqa_tree_decode(const gqa_tree_decode_params* p);
+
+/*
+ * Verification of drafted tokens against the target's probabilities, from given random numbers, so
+ * that the accepted tokens followed by next_token are distributed as the target's own samples when each
+ * node's token was drawn from the draft's row at its parent. Row n of target / draft [batch, tokens,
+ * vocab] is the distribution of the token AFTER node n. The walk starts at node 0; at node `cur`
+ * its children are tried in index order. With p, q the rows at cur, x the child's token and, before
+ * the first rejection, c = 0 and S = 1:
+ *     accept when u_accept[child] * q(x) * S < max(p(x) - c q(x), 0)       -> cur = child, c = 0, S = 1
+ *     else c += S, then S = sum_v max(p(v) - c q(v), 0)                    -> the next child
+ * (max(p - c q, 0) / S is the residual distribution of the rejections so far: the residual of a
+ * residual keeps that form.) At a node without an accepted child, next_token is the smallest v whose
+ * cumulative residual exceeds u_sample * S; if the residual is empty, p itself is used. draft null: the
+ * draft was not sampled; q is 1 at the child's token and 0 elsewhere, so a rejection removes that token
+ * from p. Entries that are negative or NaN count as 0. All sums and tests are FP64.
+ *   dtype            of target and draft: GQA_DTYPE_F32 or GQA_DTYPE_BF16.
+ *   *_seq_stride, *_node_stride   elements between sequences and between rows (0: packed).
+ *   tokens_dev, parents_dev       [batch, tokens]; a node whose parent is not before it or whose
+ *                    token is outside the vocabulary is never accepted (and sets *status_dev).
+ *   path [batch, tokens]   nodes of the accepted path, node 0 first, then -1.
+ *   kept [batch]           their number (1 .. n_b; 0 for an empty or skipped sequence).
+ *   next_token [batch]     the sampled token (-1 for an empty or skipped sequence, or a row of zeros).
+ */
+typedef struct gqa_tree_verify_params {
+    int32_t dtype;
+    int32_t batch;
+    int32_t tokens;
+    int32_t vocab;
+    int64_t target_seq_stride;
+    int64_t target_node_stride;
+    int64_t draft_seq_stride;
+    int64_t draft_node_stride;
+    const void* target;
+    const void* draft;             /* or null */
+    const int32_t* tokens_dev;
+    const int32_t* parents_dev;
+    const float* u_accept;         /* [batch, tokens], in [0, 1) */
+    const float* u_sample;         /* [batch], in [0, 1) */
+    const int32_t* tree_sizes_dev; /* [batch] or null */
+    int32_t* path;
+    int32_t* kept;
+    int32_t* next_token;
+    int32_t* status_dev;
+    void* stream;
+} gqa_tree_verify_params;
+
+int gqa_tree_verify(const gqa_tree_verify_params* p);
+
+/*
+ * Keeps the accepted path: in every layer, the K and V rows of slot seq_len - n_b + path[b, i] move to
+ * slot seq_len - n_b + i for i < kept[b], in place, and seq_lens_out[b] = seq_len - n_b + kept[b].
+ * path must ascend (path[i] > path[i - 1], path[i] < n_b), as gqa_tree_verify leaves it; a sequence whose
+ * path does not, or whose kept is outside 0 .. n_b, is skipped with its length unchanged
+ * (GQA_STATUS_BAD_INPUT). Slots behind the kept rows are left as they are.
+ *   dtype            GQA_DTYPE_BF16 or GQA_DTYPE_F32 (rows are moved bit for bit).
+ *   num_layers, layer_stride   the caches of layer l start l * layer_stride elements behind k_cache /
+ *                    v_cache; layout and block table are the same for all layers.
+ *   seq_lens_out     must not be seq_lens_dev: other blocks of the launch still read that.
+ */
+typedef struct gqa_tree_commit_params {
+    int32_t dtype;
+    int32_t batch;
+    int32_t tokens;
+    int32_t num_kv_heads;
+    int32_t head_dim;
+    int32_t num_layers;
+    int32_t blocks_per_seq;
+    int32_t fixed_block;
+    gqa_kv_layout layout;
+    int64_t layer_stride;
+    void* k_cache;
+    void* v_cache;
+    const int32_t* path;           /* [batch, tokens] */
+    const int32_t* kept;           /* [batch] */
+    const int32_t* seq_lens_dev;   /* [batch] */
+    const int32_t* tree_sizes_dev; /* [batch] or null */
+    const int32_t* block_table_dev;
+    int32_t* seq_lens_out;         /* [batch] */
+    int32_t* status_dev;
+    void* stream;
+} gqa_tree_commit_params;
+
+int gqa_tree_commit(const gqa_tree_commit_params* p);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,7 +27,14 @@ from .binding import (  # noqa: F401
     qk_norm_rope_append,
     qkv_gemv,
     qkv_workspace,
+    rope_append,
+    rope_frequencies,
     shard_plan,
     sin_cos_cache,
     status_string,
+    tree_commit,
+    tree_decode,
+    tree_masks,
+    tree_verify,
+    tree_workspace,
 )

@@ -167,6 +167,119 @@ class _QkvParams(C.Structure):
     ]
 
 
+class _RopeParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("num_q_heads", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("rotary_dim", C.c_int32),
+        ("style", C.c_int32),
+        ("blocks_per_seq", C.c_int32),
+        ("fixed_block", C.c_int32),
+        ("eps", C.c_float),
+        ("attn_factor", C.c_float),
+        ("layout", _Layout),
+        ("q_token_stride", C.c_int64),
+        ("q_out_token_stride", C.c_int64),
+        ("k_token_stride", C.c_int64),
+        ("v_token_stride", C.c_int64),
+        ("q", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("k_new", C.c_void_p),
+        ("v_new", C.c_void_p),
+        ("qk_weight", C.c_void_p),
+        ("freq_dev", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("seq_lens_dev", C.c_void_p),
+        ("tree_sizes_dev", C.c_void_p),
+        ("depth_dev", C.c_void_p),
+        ("block_table_dev", C.c_void_p),
+        ("status_dev", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class _TreeDecodeParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("num_q_heads", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("blocks_per_seq", C.c_int32),
+        ("fixed_block", C.c_int32),
+        ("layout", _Layout),
+        ("q_token_stride", C.c_int64),
+        ("q", C.c_void_p),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("out", C.c_void_p),
+        ("mask_dev", C.c_void_p),
+        ("seq_lens_dev", C.c_void_p),
+        ("tree_sizes_dev", C.c_void_p),
+        ("block_table_dev", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("status_dev", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class _TreeVerifyParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("vocab", C.c_int32),
+        ("target_seq_stride", C.c_int64),
+        ("target_node_stride", C.c_int64),
+        ("draft_seq_stride", C.c_int64),
+        ("draft_node_stride", C.c_int64),
+        ("target", C.c_void_p),
+        ("draft", C.c_void_p),
+        ("tokens_dev", C.c_void_p),
+        ("parents_dev", C.c_void_p),
+        ("u_accept", C.c_void_p),
+        ("u_sample", C.c_void_p),
+        ("tree_sizes_dev", C.c_void_p),
+        ("path", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("next_token", C.c_void_p),
+        ("status_dev", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
+class _TreeCommitParams(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("num_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("num_layers", C.c_int32),
+        ("blocks_per_seq", C.c_int32),
+        ("fixed_block", C.c_int32),
+        ("layout", _Layout),
+        ("layer_stride", C.c_int64),
+        ("k_cache", C.c_void_p),
+        ("v_cache", C.c_void_p),
+        ("path", C.c_void_p),
+        ("kept", C.c_void_p),
+        ("seq_lens_dev", C.c_void_p),
+        ("tree_sizes_dev", C.c_void_p),
+        ("block_table_dev", C.c_void_p),
+        ("seq_lens_out", C.c_void_p),
+        ("status_dev", C.c_void_p),
+        ("stream", C.c_void_p),
+    ]
+
+
 _SIGNATURES = {
     "gqa_status_string": (C.c_char_p, [C.c_int]),
     "gqa_abi_version": (C.c_int, []),
@@ -222,6 +335,15 @@ _SIGNATURES = {
     "gqa_qkv_gemv": (C.c_int, [C.POINTER(_QkvParams)]),
     "gqa_oproj_residual": (C.c_int, [C.POINTER(_OprojParams)]),
     "gqa_oproj_residual_sharded": (C.c_int, [C.POINTER(_OprojParams), C.c_void_p]),
+    "gqa_tree_masks": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p,
+                                 C.c_void_p]),
+    "gqa_rope_frequencies": (C.c_int, [C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_int32,
+                                       C.c_double, C.c_double, C.c_void_p, C.POINTER(C.c_float)]),
+    "gqa_rope_append": (C.c_int, [C.POINTER(_RopeParams)]),
+    "gqa_tree_workspace_bytes": (C.c_size_t, [C.c_int32] * 6),
+    "gqa_tree_decode": (C.c_int, [C.POINTER(_TreeDecodeParams)]),
+    "gqa_tree_verify": (C.c_int, [C.POINTER(_TreeVerifyParams)]),
+    "gqa_tree_commit": (C.c_int, [C.POINTER(_TreeCommitParams)]),
 }
 
 _lib: Optional[C.CDLL] = None
@@ -778,3 +900,246 @@ def qkv_gemv(x: torch.Tensor, weight: torch.Tensor, q_out: torch.Tensor, k_out: 
         p.workspace, p.workspace_bytes = _ptr(workspace), workspace.numel() * workspace.element_size()
     p.status_dev, p.stream = _ptr(status), stream
     _check(lib().gqa_qkv_gemv(C.byref(p)), "gqa_qkv_gemv")
+
+
+# ---- tree-drafted decoding --------------------------------------------------------------------
+
+TREE_MAX_TOKENS = 128
+ROPE_STYLES = {"half": 0, "interleaved": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def _want(name: str, t: Optional[torch.Tensor], dtype, shape, home: int) -> Optional[int]:
+    """Address of a packed device tensor of this dtype and shape (None stays None). A tensor on
+    another device than the current one, whose stream the call would use, is refused."""
+    if t is None:
+        return None
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    if t.get_device() != home:
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: not contiguous")
+    return t.data_ptr()
+
+
+def _token_rows(name: str, t: torch.Tensor, dtype, home: int):
+    """Address and token stride of [batch, tokens, heads, 128] rows whose tokens may lie apart."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if t.get_device() != home:
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
+    batch, tokens, heads, dim = t.shape
+    sb, st, sh, sd = t.stride()
+    if tokens == 1:
+        st = sb
+    if not (sd == 1 and (sh == dim or heads == 1) and (sb == tokens * st or batch == 1)) or (
+            batch * tokens > 1 and st < heads * dim):
+        raise ValueError(f"{name}: heads must be packed and sequences `tokens` token strides apart")
+    return t.data_ptr(), (st if batch * tokens > 1 else heads * dim)
+
+
+def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, home: int):
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dtype != dtype:
+            raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+        if t.get_device() != home:
+            raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
+    return k_cache.data_ptr(), v_cache.data_ptr()
+
+
+def tree_masks(parents: torch.Tensor, sizes: Optional[torch.Tensor] = None):
+    """Mask rows (int32 words [batch, tokens, ceil(tokens / 32)]) and depths [batch, tokens] of
+    trees given by their parents [batch, tokens] (-1 at node 0). Host tensors in and out."""
+    parents = parents.to(dtype=torch.int32, device="cpu").contiguous()
+    batch, tokens = parents.shape
+    if sizes is not None:
+        sizes = sizes.to(dtype=torch.int32, device="cpu").contiguous()
+        if tuple(sizes.shape) != (batch,):
+            raise ValueError(f"sizes: shape {tuple(sizes.shape)}, expected {(batch,)}")
+    mask = torch.zeros(batch, tokens, (tokens + 31) // 32, dtype=torch.int32)
+    depth = torch.zeros(batch, tokens, dtype=torch.int32)
+    _check(lib().gqa_tree_masks(_ptr(parents), _ptr(sizes), batch, tokens, _ptr(mask), _ptr(depth)),
+           "gqa_tree_masks")
+    return mask, depth
+
+
+def rope_frequencies(rotary_dim: int = 128, base: float = 1e6, scaling: str = "none",
+                     factor: float = 1.0, original_len: int = 0, beta_fast: float = 32.0,
+                     beta_slow: float = 1.0):
+    """Radians per position of each rotated pair (FP64, on the host) and the attention factor."""
+    freq = torch.zeros(max(rotary_dim // 2, 1), dtype=torch.float64)
+    attn = C.c_float()
+    _check(lib().gqa_rope_frequencies(rotary_dim, base, ROPE_SCALINGS[scaling], factor, original_len,
+                                      beta_fast, beta_slow, _ptr(freq), C.byref(attn)),
+           "gqa_rope_frequencies")
+    return freq, attn.value
+
+
+def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor,
+                v_cache: torch.Tensor, *, layout: KvLayout, seq_lens_dev: torch.Tensor,
+                freq: torch.Tensor, q_out: Optional[torch.Tensor] = None, style: str = "half",
+                attn_factor: float = 1.0, qk_weight: Optional[torch.Tensor] = None,
+                eps: float = 1e-6, depth: Optional[torch.Tensor] = None,
+                tree_sizes: Optional[torch.Tensor] = None,
+                block_table: Optional[torch.Tensor] = None, fixed_block: int = 0,
+                status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
+    """Rotates the nodes' queries q [batch, tokens, heads, 128] into q_out (q itself if None) and
+    their keys into the cache, and appends their values. `freq` (FP64, on the device, one per rotated
+    pair) comes from rope_frequencies(); tokens of q, k_new and v_new may lie apart (views of a
+    packed QKV row)."""
+    home = torch.cuda.current_device()
+    batch, tokens, hq, dim = q.shape
+    dtype = q.dtype
+    p = _RopeParams()
+    p.dtype, p.batch, p.tokens = _dtype_code(q), batch, tokens
+    p.num_q_heads, p.num_kv_heads, p.head_dim = hq, k_new.shape[2], dim
+    p.rotary_dim, p.style = 2 * freq.shape[0], ROPE_STYLES[style]
+    p.fixed_block, p.eps, p.attn_factor = fixed_block, eps, attn_factor
+    p.layout = layout.c()
+    p.q, p.q_token_stride = _token_rows("q", q, dtype, home)
+    if q_out is None:
+        p.q_out, p.q_out_token_stride = p.q, p.q_token_stride
+    else:
+        if q_out.shape != q.shape:
+            raise ValueError(f"q_out: shape {tuple(q_out.shape)}, expected {tuple(q.shape)}")
+        p.q_out, p.q_out_token_stride = _token_rows("q_out", q_out, dtype, home)
+    rows = (batch, tokens, k_new.shape[2], dim)
+    if tuple(k_new.shape) != rows or tuple(v_new.shape) != rows:
+        raise ValueError(f"k_new, v_new: shapes {tuple(k_new.shape)}, {tuple(v_new.shape)}, expected {rows}")
+    p.k_new, p.k_token_stride = _token_rows("k_new", k_new, dtype, home)
+    p.v_new, p.v_token_stride = _token_rows("v_new", v_new, dtype, home)
+    p.qk_weight = _want("qk_weight", qk_weight, dtype, (2 * dim,), home)
+    p.freq_dev = _want("freq", freq, torch.float64, None, home)
+    p.k_cache, p.v_cache = _cache_pair(k_cache, v_cache, dtype, home)
+    p.seq_lens_dev = _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home)
+    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
+    p.depth_dev = _want("depth", depth, torch.int32, (batch, tokens), home)
+    if block_table is not None:
+        p.blocks_per_seq = block_table.shape[1]
+        p.block_table_dev = _want("block_table", block_table, torch.int32,
+                                  (batch, block_table.shape[1]), home)
+    p.status_dev = _want("status", status, torch.int32, None, home)
+    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    _check(lib().gqa_rope_append(C.byref(p)), "gqa_rope_append")
+
+
+def tree_workspace(batch: int, tokens: int, num_q_heads: int, num_kv_heads: int, device,
+                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """Scratch for tree_decode (one per stream that may run at the same time)."""
+    code = DTYPE_F32 if dtype == torch.float32 else DTYPE_BF16
+    nbytes = lib().gqa_tree_workspace_bytes(code, batch, tokens, num_q_heads, num_kv_heads, 0)
+    if nbytes == 0:
+        raise ValueError("tree_workspace: unsupported shape")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def tree_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor, *,
+                num_kv_heads: int, layout: KvLayout, seq_lens_dev: torch.Tensor,
+                mask: Optional[torch.Tensor] = None, tree_sizes: Optional[torch.Tensor] = None,
+                block_table: Optional[torch.Tensor] = None, fixed_block: int = 0,
+                workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                stream: Optional[int] = None) -> None:
+    """Attention of the nodes q [batch, tokens, heads, 128] over the cached history and the nodes
+    their mask rows name (tree_masks(), on the device; None: a causal run) into `out` (packed)."""
+    home = torch.cuda.current_device()
+    batch, tokens, hq, dim = q.shape
+    p = _TreeDecodeParams()
+    p.dtype, p.batch, p.tokens = _dtype_code(q), batch, tokens
+    p.num_q_heads, p.num_kv_heads, p.head_dim = hq, num_kv_heads, dim
+    p.fixed_block = fixed_block
+    p.layout = layout.c()
+    p.q, p.q_token_stride = _token_rows("q", q, q.dtype, home)
+    p.k_cache, p.v_cache = _cache_pair(k_cache, v_cache, q.dtype, home)
+    p.out = _want("out", out, q.dtype, (batch, tokens, hq, dim), home)
+    p.mask_dev = _want("mask", mask, torch.int32, (batch, tokens, (tokens + 31) // 32), home)
+    p.seq_lens_dev = _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home)
+    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
+    if block_table is not None:
+        p.blocks_per_seq = block_table.shape[1]
+        p.block_table_dev = _want("block_table", block_table, torch.int32,
+                                  (batch, block_table.shape[1]), home)
+    if workspace is not None:
+        p.workspace = _want("workspace", workspace, torch.uint8, None, home)
+        p.workspace_bytes = workspace.numel()
+    p.status_dev = _want("status", status, torch.int32, None, home)
+    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    _check(lib().gqa_tree_decode(C.byref(p)), "gqa_tree_decode")
+
+
+def _prob_rows(name: str, t: torch.Tensor, dtype, shape, home: int):
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    if t.get_device() != home:
+        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
+    if t.stride(2) != 1 and shape[2] != 1:
+        raise ValueError(f"{name}: the vocabulary must be packed")
+    if (t.stride(0) == 0 and shape[0] > 1) or (t.stride(1) == 0 and shape[1] > 1):
+        raise ValueError(f"{name}: rows that share memory (expanded) are not supported")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def tree_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor,
+                parents: torch.Tensor, u_accept: torch.Tensor, u_sample: torch.Tensor, *,
+                path: torch.Tensor, kept: torch.Tensor, next_token: torch.Tensor,
+                tree_sizes: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                stream: Optional[int] = None) -> None:
+    """Verifies drafted `tokens` [batch, nodes] against target probabilities [batch, nodes, vocab]
+    (row n: after node n) with the draft's probabilities (or None: drafts that were not sampled)
+    and uniform numbers in [0, 1); leaves the accepted path, its length and the next token."""
+    home = torch.cuda.current_device()
+    batch, nodes, vocab = target.shape
+    p = _TreeVerifyParams()
+    p.dtype, p.batch, p.tokens, p.vocab = _dtype_code(target), batch, nodes, vocab
+    p.target, p.target_seq_stride, p.target_node_stride = _prob_rows(
+        "target", target, target.dtype, (batch, nodes, vocab), home)
+    if draft is not None:
+        p.draft, p.draft_seq_stride, p.draft_node_stride = _prob_rows(
+            "draft", draft, target.dtype, (batch, nodes, vocab), home)
+    p.tokens_dev = _want("tokens", tokens, torch.int32, (batch, nodes), home)
+    p.parents_dev = _want("parents", parents, torch.int32, (batch, nodes), home)
+    p.u_accept = _want("u_accept", u_accept, torch.float32, (batch, nodes), home)
+    p.u_sample = _want("u_sample", u_sample, torch.float32, (batch,), home)
+    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
+    p.path = _want("path", path, torch.int32, (batch, nodes), home)
+    p.kept = _want("kept", kept, torch.int32, (batch,), home)
+    p.next_token = _want("next_token", next_token, torch.int32, (batch,), home)
+    p.status_dev = _want("status", status, torch.int32, None, home)
+    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    _check(lib().gqa_tree_verify(C.byref(p)), "gqa_tree_verify")
+
+
+def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: int,
+                layout: KvLayout, seq_lens_dev: torch.Tensor, path: torch.Tensor,
+                kept: torch.Tensor, seq_lens_out: torch.Tensor, layers: int = 1,
+                layer_stride: Optional[int] = None, tree_sizes: Optional[torch.Tensor] = None,
+                block_table: Optional[torch.Tensor] = None, fixed_block: int = 0,
+                status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
+    """Moves the accepted path's K and V rows to the first of the draft's cache slots in `layers`
+    caches that lie layer_stride elements apart (default: the tensors cut in `layers` equal parts)
+    and leaves the new lengths in seq_lens_out (another tensor than seq_lens_dev)."""
+    home = torch.cuda.current_device()
+    batch, nodes = path.shape
+    p = _TreeCommitParams()
+    p.dtype, p.batch, p.tokens = _dtype_code(k_cache), batch, nodes
+    p.num_kv_heads, p.head_dim, p.num_layers = num_kv_heads, 128, layers
+    p.fixed_block = fixed_block
+    p.layout = layout.c()
+    p.layer_stride = k_cache.numel() // layers if layer_stride is None else layer_stride
+    p.k_cache, p.v_cache = _cache_pair(k_cache, v_cache, k_cache.dtype, home)
+    p.path = _want("path", path, torch.int32, (batch, nodes), home)
+    p.kept = _want("kept", kept, torch.int32, (batch,), home)
+    p.seq_lens_dev = _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home)
+    p.seq_lens_out = _want("seq_lens_out", seq_lens_out, torch.int32, (batch,), home)
+    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
+    if block_table is not None:
+        p.blocks_per_seq = block_table.shape[1]
+        p.block_table_dev = _want("block_table", block_table, torch.int32,
+                                  (batch, block_table.shape[1]), home)
+    p.status_dev = _want("status", status, torch.int32, None, home)
+    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
+    _check(lib().gqa_tree_commit(C.byref(p)), "gqa_tree_commit")

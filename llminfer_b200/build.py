@@ -29,9 +29,14 @@ KERNEL_SOURCES = [
     "csrc/kv_pool.cpp",
     "csrc/shard_comm.cu",
     "csrc/proj.cu",
+    "csrc/rope_append.cu",
+    "csrc/tree_host.cpp",
+    "csrc/tree_decode.cu",
+    "csrc/tree_verify.cu",
+    "csrc/tree_commit.cu",
 ]
 KERNEL_HEADERS = ["csrc/ptx.cuh", "csrc/work_map.cuh", "csrc/decode_kernels.cuh",
-                  "csrc/peer_window.cuh", "csrc/front_math.cuh"]
+                  "csrc/peer_window.cuh", "csrc/front_math.cuh", "csrc/tree_common.cuh"]
 
 
 def _stale(output: Path, inputs: list[Path]) -> bool:

@@ -15,6 +15,7 @@
 
 #include "decode_kernels.cuh"
 #include "peer_window.cuh"
+#include "tree_common.cuh"
 #include "work_map.cuh"
 
 namespace {
@@ -922,6 +923,63 @@ int decode_impl(const gqa_decode_params* p, const gqa_fused_front* front,
 }
 
 }  // namespace
+
+int gqa::current_sm_count(int32_t* out) { return device_sm_count(out); }
+
+int gqa::tree_cache_args(const TreeCacheDesc& d, TreeCache* out) {
+    if (d.dtype != GQA_DTYPE_F32 && d.dtype != GQA_DTYPE_BF16) return GQA_ERR_DTYPE;
+    if (d.batch <= 0 || d.tokens <= 0 || d.num_kv_heads <= 0) return GQA_ERR_SHAPE;
+    if (d.tokens > kTreeMaxTokens || d.head_dim != kHeadDim) return GQA_ERR_SHAPE;
+    const gqa_kv_layout& l = *d.layout;
+    const int rc = validate_layout(l, d.dtype, d.num_kv_heads);
+    if (rc != GQA_OK) return rc;
+    if (d.k_cache == nullptr || d.v_cache == nullptr || d.seq_lens_dev == nullptr) return GQA_ERR_NULL;
+    if (!aligned16(d.k_cache) || !aligned16(d.v_cache)) return GQA_ERR_ALIGN;
+    int64_t capacity = l.block_tokens;
+    if (d.block_table_dev != nullptr) {
+        if (d.blocks_per_seq <= 0) return GQA_ERR_SHAPE;
+        if (d.blocks_per_seq > 1 && l.block_tokens % kChunkKeys != 0) return GQA_ERR_SHAPE;
+        capacity *= d.blocks_per_seq;
+        if (capacity > INT32_MAX) return GQA_ERR_SHAPE;
+    } else {
+        if (d.batch != 1) return GQA_ERR_SHAPE;
+        if (d.fixed_block < 0 || d.fixed_block >= l.num_blocks) return GQA_ERR_RANGE;
+    }
+    out->seq_lens = d.seq_lens_dev;
+    out->tree_sizes = d.tree_sizes_dev;
+    out->block_table = d.block_table_dev;
+    out->status = d.status_dev;
+    out->stride_block = l.stride_block;
+    out->stride_token = l.stride_token;
+    out->stride_head = l.stride_head;
+    out->tokens = d.tokens;
+    out->blocks_per_seq = d.blocks_per_seq;
+    out->block_tokens = l.block_tokens;
+    out->fixed_block = d.fixed_block;
+    out->num_blocks = l.num_blocks;
+    out->capacity = (int32_t)capacity;
+    return GQA_OK;
+}
+
+int gqa::tree_cache_map(const void* base, const gqa_kv_layout& l, int32_t num_kv_heads,
+                        int32_t box_keys, bool* head_before_token, CUtensorMap* map) {
+    return encode_cache_map(base, l, num_kv_heads, box_keys, head_before_token, map);
+}
+
+int gqa::tree_query_map(const void* base, int64_t rows, int64_t token_stride, int32_t num_q_heads,
+                        int32_t group, int32_t box_tokens, CUtensorMap* map) {
+    auto fn = encode_fn();
+    if (fn == nullptr) return GQA_ERR_CUDA;
+    cuuint64_t dims[3] = {(cuuint64_t)kHeadDim, (cuuint64_t)num_q_heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)kHeadDim * 2, (cuuint64_t)token_stride * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)box_tokens};
+    cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                          strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? GQA_OK : GQA_ERR_UNSUPPORTED;
+}
 
 extern "C" {
 
