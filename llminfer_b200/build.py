@@ -32,11 +32,13 @@ KERNEL_SOURCES = [
     "csrc/rope_append.cu",
     "csrc/tree_host.cpp",
     "csrc/tree_decode.cu",
+    "csrc/tree_attention.cu",
     "csrc/tree_verify.cu",
     "csrc/tree_commit.cu",
 ]
 KERNEL_HEADERS = ["csrc/ptx.cuh", "csrc/work_map.cuh", "csrc/decode_kernels.cuh",
-                  "csrc/peer_window.cuh", "csrc/front_math.cuh", "csrc/tree_common.cuh"]
+                  "csrc/peer_window.cuh", "csrc/front_math.cuh", "csrc/tree_common.cuh",
+                  "csrc/tree_attention.cuh", "csrc/tcgen05.cuh"]
 
 
 def _stale(output: Path, inputs: list[Path]) -> bool:

@@ -1,0 +1,846 @@
+// Tree attention on the 5th-generation tensor cores (gqa_tree_decode, BF16).
+//
+// Mathematics. For a KV head the queries of up to 16 .. 128 nodes times the group form tiles of 128 rows;
+// a tile of keys is 128 positions of the cache. S = Q K^T and O += P V run as 128 x 128 x 128 products with
+// FP32 accumulators in tensor memory, P = 2^(c (S - m)) with the running maximum m and sum l in FP32
+// registers, one thread per row. P is rounded to BF16 for the second product (V is BF16 and both operands
+// have one type); the sum takes the unrounded weights. m is only moved when a tile's maximum exceeds it by 2^8:
+// the weights then stay below 2^8, their relative rounding is the same, and O (in tensor memory) is
+// rescaled a few times per sequence instead of once per tile.
+//
+// A CTA has two streams of softmax, a warpgroup each. With one query tile (rows <= 128) the streams
+// take the key tiles in turn, each with its own O, m and l, merged at the end; with two query tiles they
+// share every key tile. While one stream computes weights, the tensor cores work for the other:
+//   S(j) .. weights(j) .. O += P(j) V, then S(j + 2) of the same stream, whose S and P share columns.
+// Warps 0-7: softmax, warp 8: bulk copies of Q, K and V into 128-byte swizzled rows (a ring of 32 KiB
+// tiles), warp 9: its lane 0 issues the products.
+//
+// Work. All units (sequence, KV head, run of tokens) put their key tiles in one flat sequence that is cut evenly
+// over one CTA per SM, whatever the lengths are: few rows over a long history fill the GPU as well as
+// a ragged batch does. A piece that is a whole unit writes the output; other pieces leave (O, m, l) as
+// a record, at most two per CTA, merged by tree_merge_kernel.
+//
+// Masks. Keys before the nodes are seen by every row; only tiles that reach the nodes look at the mask (a
+// 128-bit window per row). Scores of unseen keys are replaced, not added to, so that K may hold anything there. V
+// rows past the end are zeroed in shared memory (0 * NaN). A node's V row that holds an infinity or
+// NaN is zeroed too, and added by hand to the rows that see it, in the epilogue.
+#include <cuda_bf16.h>
+
+#include <cstring>
+#include <mutex>
+
+#include "ptx.cuh"
+#include "tcgen05.cuh"
+#include "tree_attention.cuh"
+
+namespace gqa {
+namespace {
+
+constexpr int kTile = 128;                      // keys per tile, rows per query tile
+constexpr int kTileBytes = kTile * kHeadDim * 2;
+constexpr int kHalfBytes = kTileBytes / 2;      // 64 channels
+constexpr int kSlots = 6;                       // query tiles and ring together
+constexpr int kSoftmaxThreads = 256;
+constexpr int kThreads = kSoftmaxThreads + 64;
+constexpr int kUnitPad = 1;                     // places a unit counts on top of its tiles
+constexpr float kLazyMax = 8.0f;                // log2 of how far a score may exceed m
+constexpr uint64_t kWaitNs = 2000000000ull;
+constexpr uint32_t kColS = 0, kColO = 256;      // tensor memory: S0, S1, O0, O1 of 128 columns
+constexpr uint32_t kColumns = 512;
+constexpr int kRecordCols = kHeadDim + 2;
+
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Waits with a time limit; also gives up when another role has (its arrivals will not come).
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int* dead) {
+    if (mbar_try_wait(bar, parity)) return true;
+    uint64_t start = 0;
+    for (uint32_t tries = 1;; ++tries) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((tries & 255u) == 0) {
+            const uint64_t t = now_ns();
+            if (start == 0) start = t;
+            if (*dead || t - start > kWaitNs) {
+                *dead = 1;
+                return false;
+            }
+        }
+    }
+}
+
+// The same by a whole warp: one answer, and the lanes together again.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
+    return __all_sync(0xffffffffu, wait_bar(bar, parity, dead));
+}
+
+// Barrier 1 of the softmax warps: true when all of them say so.
+__device__ __forceinline__ bool meet(bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, 1, %2, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)ok), "n"(kSoftmaxThreads)
+        : "memory");
+    return all != 0;
+}
+
+// ---- the flat sequence of key tiles -------------------------------------------------------------
+struct Tables {
+    int32_t* len;   // [batch] keys (0: nothing to do)
+    int32_t* n;     // [batch] nodes
+    int32_t* base;  // [batch + 1] places before the sequence
+};
+__device__ __forceinline__ Tables tables_at(int32_t* smem, int batch) {
+    return Tables{smem, smem + batch, smem + 2 * batch};
+}
+size_t table_bytes(int batch) { return (3 * (size_t)batch + 1) * sizeof(int32_t); }
+
+template <int QT>  // query tiles per unit
+__device__ __forceinline__ int units_of(const TreeArgs& a, int n) {
+    return a.num_kv_heads * ceil_div(n, a.tile_tokens * QT);
+}
+__device__ __forceinline__ int places_of(int len) { return ceil_div(len, kTile) + kUnitPad; }
+
+// All threads of the block.
+template <int QT>
+__device__ void build_tables(const TreeArgs& a, const Tables& t) {
+    for (int b = threadIdx.x; b < a.batch; b += blockDim.x) {
+        const TreeSpan s = tree_span(a.cache, b);
+        if (!s.ok && blockIdx.x == 0) raise_bad_input(a.cache.status);
+        t.n[b] = s.n;
+        t.len[b] = s.n > 0 ? s.base + s.n : 0;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int per = ceil_div(a.batch, 32);
+        const int lo = min(a.batch, (int)threadIdx.x * per), hi = min(a.batch, lo + per);
+        int sum = 0;
+        for (int b = lo; b < hi; ++b) sum += t.n[b] > 0 ? places_of(t.len[b]) * units_of<QT>(a, t.n[b]) : 0;
+        int incl = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, d);
+            if ((int)threadIdx.x >= d) incl += up;
+        }
+        int run = incl - sum;
+        for (int b = lo; b < hi; ++b) {
+            t.base[b] = run;
+            run += t.n[b] > 0 ? places_of(t.len[b]) * units_of<QT>(a, t.n[b]) : 0;
+        }
+        if (threadIdx.x == 31) t.base[a.batch] = incl;
+    }
+    __syncthreads();
+}
+
+// CTAs that take part (none without a place), first place of CTA c, CTA that holds a place.
+__device__ __forceinline__ int used_ctas(const TreeArgs& a, int total) { return min(a.ctas, total); }
+__device__ __forceinline__ int cut_at(int c, int total, int ctas) {
+    return (int)((int64_t)min(c, ctas) * total / max(ctas, 1));
+}
+__device__ __forceinline__ int owner_of(int place, int total, int ctas) {
+    return (int)((((int64_t)place + 1) * ctas - 1) / total);
+}
+
+struct Unit {
+    int b;
+    int hk;
+    int token0;  // first node
+    int tokens;  // nodes
+    int len;     // keys, the tree's nodes among them
+    int n;       // the tree's nodes
+    int place;   // first place of the unit
+    int tiles;   // key tiles, at places place + kUnitPad ..
+};
+template <int QT>
+__device__ __forceinline__ Unit unit_at(const TreeArgs& a, const Tables& t, int place) {
+    int lo = 0, hi = a.batch;  // the last sequence that starts at or before the place
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (t.base[mid] <= place) lo = mid; else hi = mid;
+    }
+    Unit u;
+    u.b = lo;
+    u.len = t.len[lo];
+    u.n = t.n[lo];
+    const int per = places_of(u.len);
+    const int i = (place - t.base[lo]) / per;
+    const int runs = ceil_div(u.n, a.tile_tokens * QT);
+    u.hk = i / runs;
+    u.token0 = (i - u.hk * runs) * a.tile_tokens * QT;
+    u.tokens = min(u.n - u.token0, a.tile_tokens * QT);
+    u.place = t.base[lo] + i * per;
+    u.tiles = per - kUnitPad;
+    return u;
+}
+
+// A CTA's next piece at or after `pos` (moved behind it); false at the end of its range.
+struct Piece {
+    Unit u;
+    int tile;    // first key tile
+    int tiles;
+    bool whole;
+};
+template <int QT>
+__device__ __forceinline__ bool next_piece(const TreeArgs& a, const Tables& t, int* pos, int end, Piece* p) {
+    while (*pos < end) {
+        p->u = unit_at<QT>(a, t, *pos);
+        const int from = max(*pos - p->u.place - kUnitPad, 0);
+        const int to = min(end - p->u.place, p->u.tiles + kUnitPad) - kUnitPad;
+        *pos = min(end, p->u.place + p->u.tiles + kUnitPad);
+        if (to <= from) continue;  // nothing but padding
+        p->tile = from;
+        p->tiles = to - from;
+        p->whole = p->tiles == p->u.tiles;
+        return true;
+    }
+    return false;
+}
+
+// ---- order of a piece's tiles in the ring ----------------------------------------------------------
+// The first `lead` K tiles, then V(t), K(t + lead) in turn: as the products ask for them.
+struct Order {
+    int n;
+    int lead;
+    __device__ int k(int t) const { return t < lead ? t : lead + 2 * (t - lead) + 1; }
+    __device__ int v(int t) const { return min(lead, n) + t + min(t, max(n - lead, 0)); }
+};
+
+template <int QT>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                          const __grid_constant__ CUtensorMap map_v, const TreeArgs a) {
+    constexpr int kRing = kSlots - QT;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t s_kv_full[kRing], s_kv_empty[kRing], s_q_full[QT], s_q_empty[QT];
+    __shared__ uint64_t s_s_full[2], s_p_ready[2], s_o_full[2], s_o_free[2], s_drain;
+    __shared__ float s_ml[2][2][kTile];       // m (scaled, log2) and l of the streams' rows
+    __shared__ uint32_t s_bad[2][4];          // nodes with a non-finite V row, by turns of the pieces
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_dead;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                               ~static_cast<uintptr_t>(1023));
+    const uint32_t q_tiles = smem_u32(smem);
+    uint8_t* ring_ptr = smem + QT * kTileBytes;
+    const uint32_t ring = smem_u32(ring_ptr);
+    const Tables tables = tables_at(reinterpret_cast<int32_t*>(smem + kSlots * kTileBytes), a.batch);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int* dead = &s_dead;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRing; ++i) {
+            mbar_init(smem_u32(&s_kv_full[i]), 1);
+            mbar_init(smem_u32(&s_kv_empty[i]), 1);
+        }
+        for (int i = 0; i < QT; ++i) {
+            mbar_init(smem_u32(&s_q_full[i]), 1);
+            mbar_init(smem_u32(&s_q_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&s_s_full[i]), 1);
+            mbar_init(smem_u32(&s_p_ready[i]), 4);
+            mbar_init(smem_u32(&s_o_full[i]), 1);
+            mbar_init(smem_u32(&s_o_free[i]), 8);
+        }
+        mbar_init(smem_u32(&s_drain), 1);
+        mbar_init_fence();
+        s_dead = 0;
+        for (int i = 0; i < 8; ++i) (&s_bad[0][0])[i] = 0;
+    }
+    if (warp == 8 && lane == 0) {
+        prefetch_tensormap(&map_q);
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+    }
+    if (warp == 9) tmem_alloc(smem_u32(&s_tmem), kColumns);
+    pdl_launch_dependents();
+    pdl_wait();
+    build_tables<QT>(a, tables);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+
+    const int total = tables.base[a.batch];
+    const int ctas = used_ctas(a, total);
+    int pos = cut_at(blockIdx.x, total, ctas);
+    const int pos_end = cut_at(blockIdx.x + 1, total, ctas);
+    // One query tile: the streams take key tiles in turn; two: both take every key tile.
+    auto two_tiles = [&](const Unit& u) { return QT == 2 && u.tokens > a.tile_tokens; };
+
+    if (warp == 8) {
+        // ---- bulk copies ---------------------------------------------------------------------------
+        const uint64_t policy = l2_policy_evict_first();
+        const int boxes = kTile / a.box_keys;
+        const uint32_t q_bytes = 2u * a.box_tokens * a.group * 128u;
+        uint32_t fills = 0, q_fills = 0;
+        Piece p;
+        bool ok = true;
+        while (ok && next_piece<QT>(a, tables, &pos, pos_end, &p)) {
+            const bool two = two_tiles(p.u);
+            for (int st = 0; st < (two ? 2 : 1); ++st, ++q_fills) {
+                const uint32_t slot = q_fills % QT, round = q_fills / QT;
+                if (round > 0 && !wait_warp(smem_u32(&s_q_empty[slot]), (round - 1) & 1u, dead)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    const uint32_t bar = smem_u32(&s_q_full[slot]);
+                    const int row = p.u.b * a.cache.tokens + p.u.token0 + st * a.tile_tokens;
+                    mbar_arrive_expect_tx(bar, q_bytes);
+                    for (int h = 0; h < 2; ++h) {
+                        asm volatile(
+                            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+                            " [%0], [%1, {%3, %4, %5}], [%2];"
+                            ::"r"(q_tiles + slot * kTileBytes + h * kHalfBytes),
+                            "l"(reinterpret_cast<uint64_t>(&map_q)), "r"(bar), "r"(h * 64),
+                            "r"(p.u.hk * a.group), "r"(row)
+                            : "memory");
+                    }
+                }
+            }
+            auto load = [&](const CUtensorMap* map, int t) {
+                const uint32_t slot = fills % kRing, round = fills / kRing;
+                if (round > 0 && !wait_warp(smem_u32(&s_kv_empty[slot]), (round - 1) & 1u, dead)) ok = false;
+                if (!ok) return;
+                ++fills;
+                const uint32_t bar = smem_u32(&s_kv_full[slot]);
+                if (lane == 0) mbar_arrive_expect_tx(bar, kTileBytes);
+                __syncwarp();
+                // Lane 2 i + h copies half h of the tile's i-th box.
+                if (lane < 2 * boxes) {
+                    const int box = lane >> 1, h = lane & 1;
+                    const int key = (p.tile + t) * kTile + box * a.box_keys;
+                    int blk = a.cache.num_blocks, tok = 0;  // a block past the cache reads as zeros
+                    if (key < p.u.len) {
+                        tok = key;
+                        blk = a.cache.fixed_block;
+                        if (a.cache.block_table != nullptr) {
+                            const int lb = key / a.cache.block_tokens;
+                            tok = key - lb * a.cache.block_tokens;
+                            blk = __ldg(a.cache.block_table + (int64_t)p.u.b * a.cache.blocks_per_seq + lb);
+                            if ((uint32_t)blk >= (uint32_t)a.cache.num_blocks) {
+                                raise_bad_input(a.cache.status);
+                                blk = a.cache.num_blocks;
+                            }
+                        }
+                    }
+                    tma_load_4d(ring + slot * kTileBytes + h * kHalfBytes + box * a.box_keys * 128, map, bar,
+                                h * 64, a.head_first ? p.u.hk : tok, a.head_first ? tok : p.u.hk, blk, policy);
+                }
+                __syncwarp();
+            };
+            const int lead = min(two ? 1 : 2, p.tiles);
+            for (int t = 0; t < lead && ok; ++t) load(&map_k, t);
+            for (int t = 0; t < p.tiles && ok; ++t) {
+                load(&map_v, t);
+                if (t + lead < p.tiles) load(&map_k, t + lead);
+            }
+        }
+        if (!ok) {
+            // Copies in flight land before the block ends (again with a limit).
+            if (lane == 0) {
+                volatile int fresh = 0;
+                for (uint32_t f = fills > (uint32_t)kRing ? fills - kRing : 0; f < fills; ++f) {
+                    wait_bar(smem_u32(&s_kv_full[f % kRing]), (f / kRing) & 1u, &fresh);
+                }
+                for (uint32_t f = q_fills > (uint32_t)QT ? q_fills - QT : 0; f < q_fills; ++f) {
+                    wait_bar(smem_u32(&s_q_full[f % QT]), (f / QT) & 1u, &fresh);
+                }
+            }
+            __syncwarp();
+        }
+    } else if (warp == 9) {
+        // ---- products ------------------------------------------------------------------------------
+        if (lane == 0) {
+            constexpr uint32_t kShapeS = mma_shape(kTile, kTile, false);
+            constexpr uint32_t kShapeO = mma_shape(kTile, kHeadDim, true);
+            uint32_t ring_pos = 0, q_pos = 0;
+            uint32_t jobs[2] = {0, 0}, pieces[2] = {0, 0};  // per stream, over all pieces
+            bool ok = true;
+            Piece p;
+            while (ok && next_piece<QT>(a, tables, &pos, pos_end, &p)) {
+                const bool two = two_tiles(p.u);
+                const int count = two ? 2 * p.tiles : p.tiles;  // job j: stream j & 1, key tile j or j / 2
+                const Order order = {p.tiles, two ? 1 : 2};
+                for (int st = 0; st < (two ? 2 : 1) && ok; ++st) {
+                    const uint32_t f = q_pos + st;
+                    ok = wait_bar(smem_u32(&s_q_full[f % QT]), (f / QT) & 1u, dead);
+                }
+                auto issue_s = [&](int j) {
+                    const int st = j & 1, t = two ? j >> 1 : j;
+                    const uint32_t f = ring_pos + order.k(t), slot = f % kRing;
+                    ok = ok && wait_bar(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
+                    if (!ok) return;
+                    const uint32_t q = q_tiles + ((q_pos + (two ? st : 0)) % QT) * kTileBytes;
+                    const uint32_t k = ring + slot * kTileBytes;
+#pragma unroll
+                    for (int i = 0; i < kHeadDim / 16; ++i) {
+                        const uint32_t off = (i >> 2) * kHalfBytes + (i & 3) * 32;
+                        tc_mma_ss(tmem + kColS + st * 128, smem_matrix(q + off, 16, 1024),
+                                  smem_matrix(k + off, 16, 1024), kShapeS, i > 0);
+                    }
+                    tc_commit(smem_u32(&s_s_full[st]));
+                    if (!two || st == 1) tc_commit(smem_u32(&s_kv_empty[slot]));
+                    if (j == count - 1) {
+                        for (int i = 0; i < (two ? 2 : 1); ++i) tc_commit(smem_u32(&s_q_empty[(q_pos + i) % QT]));
+                    }
+                };
+                issue_s(0);
+                if (count > 1) issue_s(1);
+                for (int j = 0; j < count && ok; ++j) {
+                    const int st = j & 1, t = two ? j >> 1 : j;
+                    const uint32_t f = ring_pos + order.v(t), slot = f % kRing;
+                    ok = wait_bar(smem_u32(&s_p_ready[st]), jobs[st] & 1u, dead) &&
+                         wait_bar(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
+                    ++jobs[st];
+                    if (ok && j < 2 && pieces[st] > 0) {  // the last piece's O has been read
+                        ok = wait_bar(smem_u32(&s_o_free[st]), (pieces[st] - 1) & 1u, dead);
+                    }
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t v = ring + slot * kTileBytes;
+#pragma unroll
+                    for (int i = 0; i < kTile / 16; ++i) {
+                        tc_mma_ts(tmem + kColO + st * 128, tmem + kColS + st * 128 + i * 8,
+                                  smem_matrix(v + i * 2048, kHalfBytes, 1024), kShapeO, j >= 2 || i > 0);
+                    }
+                    if (!two || st == 1) tc_commit(smem_u32(&s_kv_empty[slot]));
+                    if (j + 2 >= count) {
+                        tc_commit(smem_u32(&s_o_full[st]));
+                        ++pieces[st];
+                    } else {
+                        issue_s(j + 2);
+                    }
+                }
+                ring_pos += 2 * p.tiles;
+                q_pos += two ? 2 : 1;
+            }
+            if (!ok) {
+                // Products in flight finish before tensor memory is given back (with a limit).
+                volatile int fresh = 0;
+                tc_commit(smem_u32(&s_drain));
+                wait_bar(smem_u32(&s_drain), 0, &fresh);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- weights ---------------------------------------------------------------------------------
+        const int st = warp >> 2;             // stream
+        const int row = threadIdx.x & 127;    // of the stream's query tile; lane of tensor memory
+        const uint32_t my_lanes = tmem + ((uint32_t)(warp & 3) << 21);
+        const uint32_t my_s = my_lanes + kColS + st * 128;
+        const float scale = a.scale_log2;
+        const int words = (a.cache.tokens + 31) / 32;
+        uint32_t ring_pos = 0, jobs = 0, pieces[2] = {0, 0}, turn = 0;
+        bool ok = true;
+        Piece p;
+        while (ok && next_piece<QT>(a, tables, &pos, pos_end, &p)) {
+            const bool two = two_tiles(p.u);
+            const int count = two ? 2 * p.tiles : p.tiles;
+            const Order order = {p.tiles, two ? 1 : 2};
+            const int in_unit = row / a.group + (two ? st * a.tile_tokens : 0);
+            const int token = p.u.token0 + in_unit;
+            const bool live = row < a.tile_tokens * a.group && in_unit < p.u.tokens;
+            const bool any_live = __any_sync(0xffffffffu, live);
+            const int64_t mask_row = (int64_t)p.u.b * a.cache.tokens + token;
+            const int base = p.u.len - p.u.n;
+
+            // Bits of 32 keys from tree index `first` (negative: history) that this row sees.
+            auto window = [&](int first) -> uint32_t {
+                if (first <= -32) return 0xffffffffu;
+                auto word = [&](int w) -> uint32_t {  // nodes 32 w .. 32 w + 31
+                    if (w < 0) return 0xffffffffu;
+                    if (w * 32 >= p.u.n) return 0u;
+                    uint32_t bits = a.mask != nullptr ? __ldg(a.mask + mask_row * words + w)
+                                    : token >= w * 32 + 31 ? 0xffffffffu
+                                    : token < w * 32       ? 0u
+                                                           : (2u << (token - w * 32)) - 1u;
+                    if (p.u.n - w * 32 < 32) bits &= (1u << (p.u.n - w * 32)) - 1u;
+                    return bits;
+                };
+                const int w = first >> 5;  // rounds down
+                return __funnelshift_r(word(w), word(w + 1), first & 31);
+            };
+
+            float m = -INFINITY, l = 0.0f;  // m: of the raw scores
+#pragma unroll 1
+            for (int j = st; j < count && ok; j += 2, ++jobs) {
+                const int t = two ? j >> 1 : j;
+                const int key0 = (p.tile + t) * kTile;
+                ok = wait_warp(smem_u32(&s_s_full[st]), jobs & 1u, dead);
+                if (!ok) break;
+                tc_fence_after();
+                const bool tail = key0 + kTile > base;
+                if (any_live) {
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_load32(my_s + 32 * c, s[c]);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
+                    if (tail) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t sees = live ? window(key0 + 32 * c - base) : 0u;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                if (!(sees >> i & 1u)) s[c][i] = 0xff800000u;
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                        for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                    }
+                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    if (j < 2) {
+                        m = mx;
+                    } else {
+                        const bool grow = (mx - m) * scale > kLazyMax || (m == -INFINITY && mx > m);
+                        if (__any_sync(0xffffffffu, grow)) {
+                            // S(j) was issued behind the product with the last P: O is at rest.
+                            const float next = grow ? mx : m;
+                            const float alpha = grow ? ex2_approx((m - next) * scale) : 1.0f;
+                            m = next;
+                            l *= alpha;
+#pragma unroll 1
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t o[32];
+                                const uint32_t at = my_lanes + kColO + st * 128 + 32 * c;
+                                tmem_load32(at, o);
+                                tmem_loaded(o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                }
+                                tmem_store32(at, o);
+                            }
+                        }
+                    }
+                    const float off = safe_max(m) * scale;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float e0 = ex2_approx(__uint_as_float(s[2 * half + c][2 * i]) * scale - off);
+                                const float e1 = ex2_approx(__uint_as_float(s[2 * half + c][2 * i + 1]) * scale - off);
+                                sum[i & 3] += e0 + e1;
+                                w[16 * c + i] = pack_bf16(e0, e1);
+                            }
+                        }
+                        tmem_store32(my_s + 32 * half, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_stored();
+                }
+                if (tail) {
+                    // V: rows past the end become zeros, rows of nodes are looked over.
+                    const uint32_t f = ring_pos + order.v(t), slot = f % kRing;
+                    ok = wait_warp(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
+                    if (!ok) break;
+                    const int key = key0 + row;
+                    uint4* v = reinterpret_cast<uint4*>(ring_ptr + slot * kTileBytes + row * 128);
+                    bool clear = key >= p.u.len;
+                    if (key >= base && !clear) {
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i) {
+                            const uint4 x = v[(i >> 3) * (kHalfBytes / 16) + (i & 7)];
+                            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                clear = clear || (e[c] & 0x7f80u) == 0x7f80u || (e[c] & 0x7f800000u) == 0x7f800000u;
+                            }
+                        }
+                        if (clear) atomicOr(&s_bad[turn & 1][(key - base) >> 5], 1u << ((key - base) & 31));
+                    }
+                    if (clear) {
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i) v[(i >> 3) * (kHalfBytes / 16) + (i & 7)] = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&s_p_ready[st]));
+            }
+            ring_pos += 2 * p.tiles;
+            // ---- the end of the piece ------------------------------------------------------------------
+            const bool active1 = count > 1;
+            ok = ok && wait_warp(smem_u32(&s_o_full[0]), pieces[0] & 1u, dead) &&
+                 (!active1 || wait_warp(smem_u32(&s_o_full[1]), pieces[1] & 1u, dead));
+            // Both warpgroups meet here, also when a wait ran out, and go on or leave together.
+            s_ml[st][0][row] = m * scale;
+            s_ml[st][1][row] = l;
+            if (threadIdx.x < 4) s_bad[(turn + 1) & 1][threadIdx.x] = 0;
+            tc_fence_before();
+            ok = meet(ok);
+            tc_fence_after();
+            if (!ok) break;
+            // Two tiles: this stream's rows, all channels. One tile: both streams' sums of the
+            // rows, merged; the warpgroups take 64 channels each.
+            float f0 = 1.0f, f1 = 0.0f, m_row, l_row;
+            if (two) {
+                m_row = s_ml[st][0][row];
+                l_row = l;
+            } else {
+                const float m0 = s_ml[0][0][row], m1 = active1 ? s_ml[1][0][row] : -INFINITY;
+                m_row = fmaxf(m0, m1);
+                f0 = ex2_approx(m0 - safe_max(m_row));
+                f1 = ex2_approx(m1 - safe_max(m_row));
+                l_row = s_ml[0][1][row] * f0 + (active1 ? s_ml[1][1][row] * f1 : 0.0f);
+            }
+            if (any_live) {
+                const int chunk0 = two ? 0 : 2 * st, chunks = two ? 4 : 2;
+                const float inv = l_row == 0.0f ? 0.0f : 1.0f / l_row;
+                const int head = p.u.hk * a.group + row % a.group;
+                __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                                     (mask_row * a.num_q_heads + head) * kHeadDim;
+                float* rec = a.workspace + ((int64_t)(2 * blockIdx.x + (p.tile == 0 ? 1 : 0)) * QT + (two ? st : 0)) *
+                                               a.tile_rows * kRecordCols;
+                uint32_t bad[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bad[i] = s_bad[turn & 1][i];
+#pragma unroll 1
+                for (int c = chunk0; c < chunk0 + chunks; ++c) {
+                    uint32_t o[32];
+                    float acc[32];
+                    tmem_load32(my_lanes + kColO + (two ? st : 0) * 128 + 32 * c, o);
+                    tmem_loaded(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) acc[i] = __uint_as_float(o[i]) * f0;
+                    if (!two && active1) {
+                        tmem_load32(my_lanes + kColO + 128 + 32 * c, o);
+                        tmem_loaded(o);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) acc[i] += __uint_as_float(o[i]) * f1;
+                    }
+                    if ((bad[0] | bad[1] | bad[2] | bad[3]) != 0 && live) {
+                        // Nodes left out of the product: their weights again, then channel by channel.
+                        for (int node = 0; node < p.u.n; ++node) {
+                            if (!(s_bad[turn & 1][node >> 5] >> (node & 31) & 1u)) continue;
+                            if (!tree_sees(a.mask, mask_row, words, token, node)) continue;
+                            int64_t at = 0;
+                            if (!tree_row(a.cache, p.u.b, base + node, &at)) continue;
+                            at += (int64_t)p.u.hk * a.cache.stride_head;
+                            const __nv_bfloat16* k = static_cast<const __nv_bfloat16*>(a.k_cache) + at;
+                            const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(a.v_cache) + at;
+                            const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) +
+                                                     mask_row * a.q_stride + head * kHeadDim;
+                            float dot = 0.0f;
+                            for (int d = 0; d < kHeadDim; ++d) dot += __bfloat162float(q[d]) * __bfloat162float(k[d]);
+                            const float w = ex2_approx(dot * scale - safe_max(m_row));
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) acc[i] += w * __bfloat162float(v[32 * c + i]);
+                        }
+                    }
+                    if (live && p.whole) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 w;
+                            w.x = pack_bf16(acc[8 * i] * inv, acc[8 * i + 1] * inv);
+                            w.y = pack_bf16(acc[8 * i + 2] * inv, acc[8 * i + 3] * inv);
+                            w.z = pack_bf16(acc[8 * i + 4] * inv, acc[8 * i + 5] * inv);
+                            w.w = pack_bf16(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv);
+                            *reinterpret_cast<uint4*>(out + 32 * c + 8 * i) = w;
+                        }
+                    } else if (live) {
+                        // [channel / 4][row][4]: a warp writes 512 contiguous bytes.
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            *reinterpret_cast<float4*>(rec + ((8 * c + i) * a.tile_rows + row) * 4) =
+                                make_float4(acc[4 * i], acc[4 * i + 1], acc[4 * i + 2], acc[4 * i + 3]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (live && !p.whole && (two || st == 0)) {
+                    rec[kHeadDim * a.tile_rows + row] = m_row;
+                    rec[(kHeadDim + 1) * a.tile_rows + row] = l_row;
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(smem_u32(&s_o_free[0]));
+                if (active1) mbar_arrive(smem_u32(&s_o_free[1]));
+            }
+            ++pieces[0];
+            if (active1) ++pieces[1];
+            ++turn;
+        }
+    }
+    __syncthreads();
+    if (s_dead && threadIdx.x == 0 && a.cache.status != nullptr) atomicExch(a.cache.status, kStatusStageTimeout);
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_free(tmem, kColumns);
+    }
+}
+
+// Merges the records of the units that were cut: out = sum_i O_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), pieces in
+// ascending order. grid.x: units, or (by_cut) the cuts between CTAs, of which the first inside a unit
+// stands for it; grid.y: groups of 8 rows. Thread: row tid % 8 of the group, channels 4 (tid / 8) .. + 3.
+template <int QT>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int by_cut) {
+    extern __shared__ int32_t s_tables[];
+    const Tables t = tables_at(s_tables, a.batch);
+    pdl_launch_dependents();
+    pdl_wait();
+    build_tables<QT>(a, t);
+    const int total = t.base[a.batch];
+    const int ctas = used_ctas(a, total);
+    Unit u;
+    if (by_cut) {
+        const int c = blockIdx.x + 1;
+        if (c >= ctas) return;
+        const int at = cut_at(c, total, ctas);
+        u = unit_at<QT>(a, t, at);
+        const int first = u.place + kUnitPad;
+        if (at <= first || cut_at(c - 1, total, ctas) > first) return;
+    } else {
+        // The blockIdx.x-th unit: the sequences' units in order.
+        int b = 0, i = blockIdx.x;
+        while (b < a.batch) {
+            const int here = t.n[b] > 0 ? units_of<QT>(a, t.n[b]) : 0;
+            if (i < here) break;
+            i -= here;
+            ++b;
+        }
+        if (b == a.batch) return;
+        u = unit_at<QT>(a, t, t.base[b] + i * places_of(t.len[b]));
+    }
+    const int lo = u.place + kUnitPad;
+    const int c0 = owner_of(lo, total, ctas), c1 = owner_of(lo + u.tiles - 1, total, ctas);
+    if (c0 == c1) return;  // whole: already written
+    const int tiles_rows = a.tile_tokens * a.group;
+    const int r = blockIdx.y * 8 + (threadIdx.x & 7);  // row of the unit
+    if (r >= u.tokens * a.group) return;
+    const int tile = r / tiles_rows, row = r - tile * tiles_rows;
+    const int chunk = threadIdx.x >> 3;
+    const int64_t record = (int64_t)QT * a.tile_rows * kRecordCols;
+    const float* rec = a.workspace + (int64_t)tile * a.tile_rows * kRecordCols;
+    auto at = [&](int c) { return rec + (int64_t)(2 * c + (c == c0 ? 1 : 0)) * record; };
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int kBatch = 8;
+    for (int c = c0; c <= c1; c += kBatch) {
+        float mi[kBatch], li[kBatch];
+        float4 oi[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            mi[i] = -INFINITY;
+            if (c + i > c1) continue;
+            const float* p = at(c + i);
+            mi[i] = p[kHeadDim * a.tile_rows + row];
+            li[i] = p[(kHeadDim + 1) * a.tile_rows + row];
+            oi[i] = *reinterpret_cast<const float4*>(p + ((int64_t)chunk * a.tile_rows + row) * 4);
+        }
+        float next = m;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) next = fmaxf(next, mi[i]);
+        const float ref = safe_max(next);
+        const float f = ex2_approx(m - ref);
+        l *= f;
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (c + i > c1) continue;
+            const float w = ex2_approx(mi[i] - ref);
+            l += li[i] * w;
+            o.x += oi[i].x * w; o.y += oi[i].y * w; o.z += oi[i].z * w; o.w += oi[i].w * w;
+        }
+        m = next;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int token = u.token0 + r / a.group;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
+                         (((int64_t)u.b * a.cache.tokens + token) * a.num_q_heads + u.hk * a.group + r % a.group) *
+                             kHeadDim + chunk * 4;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+}
+
+int query_tiles(int32_t tokens, int32_t group) { return tokens * group > kTile ? 2 : 1; }
+
+int rows_per_tile(int32_t tokens, int32_t group) {
+    const int per = kTile / group, used = tokens < per ? tokens : per;
+    return (used * group + 31) / 32 * 32;
+}
+
+template <int QT>
+int launch(const TreeArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
+           cudaStream_t stream) {
+    const size_t smem = 1024 + kSlots * kTileBytes + table_bytes(a.batch);
+    auto kernel = tree_attention_kernel<QT>;
+    {
+        static std::mutex mu;
+        static size_t configured[64] = {};
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return GQA_ERR_CUDA;
+        std::lock_guard<std::mutex> lock(mu);
+        if (configured[dev] < smem) {
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+                return GQA_ERR_CUDA;
+            }
+            configured[dev] = smem;
+        }
+    }
+    if (launch_pdl(kernel, dim3(a.ctas), dim3(kThreads), smem, stream, mq, mk, mv, a) != cudaSuccess) {
+        return GQA_ERR_CUDA;
+    }
+    const int64_t units = (int64_t)a.batch * a.num_kv_heads * ceil_div(a.cache.tokens, a.tile_tokens * QT);
+    const int by_cut = units > a.ctas ? 1 : 0;
+    const int unit_tokens = a.cache.tokens < a.tile_tokens * QT ? a.cache.tokens : a.tile_tokens * QT;
+    const dim3 grid((unsigned)(by_cut ? a.ctas - 1 : units), (unsigned)ceil_div(unit_tokens * a.group, 8));
+    if (by_cut && a.ctas < 2) return GQA_OK;
+    return launch_pdl(tree_merge_kernel<QT>, grid, dim3(256), table_bytes(a.batch), stream, a, by_cut) == cudaSuccess
+               ? GQA_OK
+               : GQA_ERR_CUDA;
+}
+
+}  // namespace
+
+size_t tree_attention_workspace(int32_t tokens, int32_t group, int32_t ctas) {
+    return (size_t)2 * ctas * query_tiles(tokens, group) * rows_per_tile(tokens, group) * kRecordCols * sizeof(float);
+}
+
+int launch_tree_attention(TreeArgs a, const gqa_kv_layout& layout, int32_t sm_count, cudaStream_t stream) {
+    a.ctas = sm_count;
+    a.tile_tokens = kTile / a.group;
+    a.tile_rows = rows_per_tile(a.cache.tokens, a.group);
+    a.box_tokens = a.cache.tokens < a.tile_tokens ? a.cache.tokens : a.tile_tokens;
+    // Bulk copies stay inside a block: the largest of 128, 64, 32 rows that divides it.
+    a.box_keys = kTile;
+    if (a.cache.block_table != nullptr && a.cache.blocks_per_seq > 1) {
+        while (layout.block_tokens % a.box_keys != 0) a.box_keys /= 2;
+    }
+    // Places are 32-bit numbers.
+    const int64_t per_seq = (int64_t)(ceil_div(a.cache.capacity, kTile) + kUnitPad) * a.num_kv_heads *
+                            ceil_div(a.cache.tokens, a.tile_tokens);
+    if (per_seq * a.batch > (1 << 30)) return GQA_ERR_SHAPE;
+    if ((int64_t)a.batch * a.cache.tokens > INT32_MAX) return GQA_ERR_SHAPE;
+    CUtensorMap mq, mk, mv;
+    bool head_first = false;
+    int rc = tree_cache_map(a.k_cache, layout, a.num_kv_heads, a.box_keys, &head_first, &mk);
+    if (rc == GQA_OK) rc = tree_cache_map(a.v_cache, layout, a.num_kv_heads, a.box_keys, &head_first, &mv);
+    if (rc == GQA_OK) {
+        rc = tree_query_map(a.q, (int64_t)a.batch * a.cache.tokens, a.q_stride, a.num_q_heads, a.group, a.box_tokens, &mq);
+    }
+    if (rc != GQA_OK) return rc;
+    a.head_first = head_first ? 1 : 0;
+    return query_tiles(a.cache.tokens, a.group) == 2 ? launch<2>(a, mq, mk, mv, stream)
+                                                     : launch<1>(a, mq, mk, mv, stream);
+}
+
+}  // namespace gqa

@@ -1,5 +1,5 @@
-// Attention of a tree of drafted tokens over the cache (gqa_tree_decode): C entry and the plain
-// streaming kernel on CUDA cores.
+// Attention of a tree of drafted tokens over the cache (gqa_tree_decode): C entry and the FP32 kernel on
+// CUDA cores (the BF16 kernel is in tree_attention.cu).
 //
 // Node t of sequence b sees the history (positions < base) and the nodes its mask row names; keys a row
 // does not see are never used, so their rows may hold anything. tree_rows_kernel: one CTA per (sequence,
@@ -12,7 +12,7 @@
 #include <cstring>
 
 #include "ptx.cuh"
-#include "tree_common.cuh"
+#include "tree_attention.cuh"
 
 namespace gqa {
 namespace {
@@ -20,45 +20,14 @@ namespace {
 constexpr int kWarps = 8;
 constexpr int kMaxGroup = 8;
 
-struct TreeArgs {
-    TreeCache cache;
-    const void* q;
-    const void* k_cache;
-    const void* v_cache;
-    void* out;
-    const uint32_t* mask;
-    int64_t q_stride;
-    int32_t num_q_heads;
-    int32_t num_kv_heads;
-    int32_t group;
-    float scale_log2;
-};
-
-// Whether node t sees node j (both below the sequence's n).
-__device__ __forceinline__ bool tree_sees(const uint32_t* mask, int64_t row, int words, int t, int j) {
-    if (mask == nullptr) return j <= t;
-    return (__ldg(mask + row * words + (j >> 5)) >> (j & 31)) & 1u;
-}
-
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    x[0] = bf16_lo_to_f32(u.x);
-    x[1] = bf16_hi_to_f32(u.x);
-    x[2] = bf16_lo_to_f32(u.y);
-    x[3] = bf16_hi_to_f32(u.y);
-}
 __device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
     const float4 u = *reinterpret_cast<const float4*>(p);
     x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-}
-__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
 }
 __device__ __forceinline__ void store4(float* p, const float (&x)[4]) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
-template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) tree_rows_kernel(const TreeArgs a) {
     __shared__ float s_q[kMaxGroup][kHeadDim];
     __shared__ float s_o[kWarps][kMaxGroup][kHeadDim];
@@ -75,7 +44,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_rows_kernel(const TreeArgs a
     const int64_t row = (int64_t)b * a.cache.tokens + t;
     for (int i = threadIdx.x; i < group * kHeadDim / 4; i += kWarps * 32) {
         float x[4];
-        load4(static_cast<const T*>(a.q) + row * a.q_stride + (int64_t)hk * group * kHeadDim + i * 4, x);
+        load4(static_cast<const float*>(a.q) + row * a.q_stride + (int64_t)hk * group * kHeadDim + i * 4, x);
 #pragma unroll
         for (int c = 0; c < 4; ++c) (&s_q[0][0])[i * 4 + c] = x[c] * a.scale_log2;
     }
@@ -102,7 +71,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_rows_kernel(const TreeArgs a
 #pragma unroll
         for (int g = 0; g < kMaxGroup; ++g) s[g] = 0.0f;
         if (sees) {
-            const T* kp = static_cast<const T*>(a.k_cache) + off;
+            const float* kp = static_cast<const float*>(a.k_cache) + off;
 #pragma unroll 4
             for (int d = 0; d < kHeadDim; d += 4) {
                 float x[4];
@@ -139,7 +108,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_rows_kernel(const TreeArgs a
             todo &= todo - 1;
             const int64_t at = __shfl_sync(0xffffffffu, off, j);
             float x[4];
-            load4(static_cast<const T*>(a.v_cache) + at + lane * 4, x);
+            load4(static_cast<const float*>(a.v_cache) + at + lane * 4, x);
 #pragma unroll
             for (int g = 0; g < kMaxGroup; ++g) {
                 if (g < group) {
@@ -177,7 +146,7 @@ __global__ void __launch_bounds__(kWarps * 32) tree_rows_kernel(const TreeArgs a
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) y[c] = sum == 0.0f ? 0.0f : y[c] / sum;
-        store4(static_cast<T*>(a.out) + (row * a.num_q_heads + (int64_t)hk * group + g) * kHeadDim + d, y);
+        store4(static_cast<float*>(a.out) + (row * a.num_q_heads + (int64_t)hk * group + g) * kHeadDim + d, y);
     }
 }
 
@@ -197,8 +166,9 @@ extern "C" {
 size_t gqa_tree_workspace_bytes(int32_t dtype, int32_t batch, int32_t tokens, int32_t num_q_heads,
                                 int32_t num_kv_heads, int32_t sm_count) {
     if (!gqa::shape_ok(dtype, batch, tokens, num_q_heads, num_kv_heads)) return 0;
-    (void)sm_count;
-    return 16;
+    if (dtype == GQA_DTYPE_F32) return 16;
+    if (sm_count <= 0 && gqa::current_sm_count(&sm_count) != GQA_OK) return 0;
+    return gqa::tree_attention_workspace(tokens, num_q_heads / num_kv_heads, sm_count);
 }
 
 int gqa_tree_decode(const gqa_tree_decode_params* p) {
@@ -238,13 +208,13 @@ int gqa_tree_decode(const gqa_tree_decode_params* p) {
     a.num_kv_heads = p->num_kv_heads;
     a.group = p->num_q_heads / p->num_kv_heads;
     a.scale_log2 = (1.0f / std::sqrt((float)kHeadDim)) * 1.44269504088896340736f;
+    a.batch = p->batch;
+    a.workspace = static_cast<float*>(p->workspace);
     if (p->num_kv_heads > 65535) return GQA_ERR_SHAPE;
-    const dim3 grid((unsigned)p->tokens, (unsigned)p->num_kv_heads, (unsigned)p->batch);
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(p->stream);
-    const cudaError_t e =
-        p->dtype == GQA_DTYPE_F32
-            ? launch_pdl(tree_rows_kernel<float>, grid, dim3(kWarps * 32), 0, stream, a)
-            : launch_pdl(tree_rows_kernel<__nv_bfloat16>, grid, dim3(kWarps * 32), 0, stream, a);
+    if (p->dtype == GQA_DTYPE_BF16) return launch_tree_attention(a, p->layout, sms, stream);
+    const dim3 grid((unsigned)p->tokens, (unsigned)p->num_kv_heads, (unsigned)p->batch);
+    const cudaError_t e = launch_pdl(tree_rows_kernel, grid, dim3(kWarps * 32), 0, stream, a);
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
