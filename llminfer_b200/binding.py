@@ -7,6 +7,7 @@ has not been built, importing it raises; if a call fails, ``GqaError`` carries t
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Optional, Sequence
@@ -339,11 +340,11 @@ _SIGNATURES = {
                                  C.c_void_p]),
     "gqa_rope_frequencies": (C.c_int, [C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_int32,
                                        C.c_double, C.c_double, C.c_void_p, C.POINTER(C.c_float)]),
-    "gqa_rope_append": (C.c_int, [C.POINTER(_RopeParams)]),
+    "gqa_rope_append": (C.c_int, [C.c_void_p]),  # _RopeParams
     "gqa_tree_workspace_bytes": (C.c_size_t, [C.c_int32] * 6),
-    "gqa_tree_decode": (C.c_int, [C.POINTER(_TreeDecodeParams)]),
-    "gqa_tree_verify": (C.c_int, [C.POINTER(_TreeVerifyParams)]),
-    "gqa_tree_commit": (C.c_int, [C.POINTER(_TreeCommitParams)]),
+    "gqa_tree_decode": (C.c_int, [C.c_void_p]),  # _TreeDecodeParams
+    "gqa_tree_verify": (C.c_int, [C.c_void_p]),  # _TreeVerifyParams
+    "gqa_tree_commit": (C.c_int, [C.c_void_p]),  # _TreeCommitParams
 }
 
 _lib: Optional[C.CDLL] = None
@@ -909,45 +910,67 @@ ROPE_STYLES = {"half": 0, "interleaved": 1}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 
-def _want(name: str, t: Optional[torch.Tensor], dtype, shape, home: int) -> Optional[int]:
-    """Address of a packed device tensor of this dtype and shape (None stays None). A tensor on
-    another device than the current one, whose stream the call would use, is refused."""
-    if t is None:
-        return None
+# The parameter blocks of the four calls as they lie in memory, packed in one go: filling a ctypes
+# structure field by field costs more host time than the kernels of a short step run.
+_ROPE = struct.Struct("@10i2f2i3q4q14P")
+_TREE_DECODE = struct.Struct("@8i2i3qq9PN2P")
+_TREE_VERIFY = struct.Struct("@4i4q12P")
+_TREE_COMMIT = struct.Struct("@8i2i3qq10P")
+
+
+def _refuse(name: str, t: torch.Tensor, dtype, shape, home: int):
     if t.dtype != dtype:
         raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
     if t.get_device() != home:
         raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: not contiguous")
+    if shape is not None and tuple(t.shape) != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
+    raise ValueError(f"{name}: not contiguous")
+
+
+def _want(name: str, t: Optional[torch.Tensor], dtype, shape, home: int) -> int:
+    """Address of a packed device tensor of this dtype and shape (0 for None). A tensor on
+    another device than the current one, whose stream the call would use, is refused."""
+    if t is None:
+        return 0
+    if (t.dtype is not dtype or (shape is not None and t.shape != shape) or t.get_device() != home
+            or not t.is_contiguous()):
+        _refuse(name, t, dtype, shape, home)
+    return t.data_ptr()
+
+
+def _on_device(name: str, t: torch.Tensor, dtype, home: int) -> int:
+    if t.dtype is not dtype or t.get_device() != home:
+        _refuse(name, t, dtype, None, home)
     return t.data_ptr()
 
 
 def _token_rows(name: str, t: torch.Tensor, dtype, home: int):
     """Address and token stride of [batch, tokens, heads, 128] rows whose tokens may lie apart."""
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if t.get_device() != home:
-        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
+    if t.dtype is not dtype or t.get_device() != home:
+        _refuse(name, t, dtype, None, home)
     batch, tokens, heads, dim = t.shape
+    if t.is_contiguous():
+        return t.data_ptr(), heads * dim
     sb, st, sh, sd = t.stride()
     if tokens == 1:
         st = sb
-    if not (sd == 1 and (sh == dim or heads == 1) and (sb == tokens * st or batch == 1)) or (
+    if sd != 1 or (sh != dim and heads != 1) or (sb != tokens * st and batch != 1) or (
             batch * tokens > 1 and st < heads * dim):
         raise ValueError(f"{name}: heads must be packed and sequences `tokens` token strides apart")
     return t.data_ptr(), (st if batch * tokens > 1 else heads * dim)
 
 
-def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, home: int):
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if t.dtype != dtype:
-            raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
-        if t.get_device() != home:
-            raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
-    return k_cache.data_ptr(), v_cache.data_ptr()
+def _table(block_table: Optional[torch.Tensor], batch: int, home: int):
+    """Address and blocks per sequence of a block table [batch, blocks_per_seq] (or None)."""
+    if block_table is None:
+        return 0, 0
+    per = block_table.shape[1]
+    return _want("block_table", block_table, torch.int32, (batch, per), home), per
+
+
+def _stream(stream: Optional[int], home: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(home) if stream is None else stream
 
 
 def tree_masks(parents: torch.Tensor, sizes: Optional[torch.Tensor] = None):
@@ -992,38 +1015,32 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
     packed QKV row)."""
     home = torch.cuda.current_device()
     batch, tokens, hq, dim = q.shape
+    hkv = k_new.shape[2]
     dtype = q.dtype
-    p = _RopeParams()
-    p.dtype, p.batch, p.tokens = _dtype_code(q), batch, tokens
-    p.num_q_heads, p.num_kv_heads, p.head_dim = hq, k_new.shape[2], dim
-    p.rotary_dim, p.style = 2 * freq.shape[0], ROPE_STYLES[style]
-    p.fixed_block, p.eps, p.attn_factor = fixed_block, eps, attn_factor
-    p.layout = layout.c()
-    p.q, p.q_token_stride = _token_rows("q", q, dtype, home)
+    q_ptr, q_stride = _token_rows("q", q, dtype, home)
     if q_out is None:
-        p.q_out, p.q_out_token_stride = p.q, p.q_token_stride
+        out_ptr, out_stride = q_ptr, q_stride
     else:
         if q_out.shape != q.shape:
             raise ValueError(f"q_out: shape {tuple(q_out.shape)}, expected {tuple(q.shape)}")
-        p.q_out, p.q_out_token_stride = _token_rows("q_out", q_out, dtype, home)
-    rows = (batch, tokens, k_new.shape[2], dim)
-    if tuple(k_new.shape) != rows or tuple(v_new.shape) != rows:
+        out_ptr, out_stride = _token_rows("q_out", q_out, dtype, home)
+    rows = (batch, tokens, hkv, dim)
+    if k_new.shape != rows or v_new.shape != rows:
         raise ValueError(f"k_new, v_new: shapes {tuple(k_new.shape)}, {tuple(v_new.shape)}, expected {rows}")
-    p.k_new, p.k_token_stride = _token_rows("k_new", k_new, dtype, home)
-    p.v_new, p.v_token_stride = _token_rows("v_new", v_new, dtype, home)
-    p.qk_weight = _want("qk_weight", qk_weight, dtype, (2 * dim,), home)
-    p.freq_dev = _want("freq", freq, torch.float64, None, home)
-    p.k_cache, p.v_cache = _cache_pair(k_cache, v_cache, dtype, home)
-    p.seq_lens_dev = _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home)
-    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
-    p.depth_dev = _want("depth", depth, torch.int32, (batch, tokens), home)
-    if block_table is not None:
-        p.blocks_per_seq = block_table.shape[1]
-        p.block_table_dev = _want("block_table", block_table, torch.int32,
-                                  (batch, block_table.shape[1]), home)
-    p.status_dev = _want("status", status, torch.int32, None, home)
-    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
-    _check(lib().gqa_rope_append(C.byref(p)), "gqa_rope_append")
+    k_ptr, k_stride = _token_rows("k_new", k_new, dtype, home)
+    v_ptr, v_stride = _token_rows("v_new", v_new, dtype, home)
+    table, per_seq = _table(block_table, batch, home)
+    _check(lib().gqa_rope_append(_ROPE.pack(
+        _dtype_code(q), batch, tokens, hq, hkv, dim, 2 * freq.shape[0], ROPE_STYLES[style], per_seq,
+        fixed_block, eps, attn_factor, layout.block_tokens, layout.num_blocks, layout.stride_block,
+        layout.stride_token, layout.stride_head, q_stride, out_stride, k_stride, v_stride, q_ptr, out_ptr,
+        k_ptr, v_ptr, _want("qk_weight", qk_weight, dtype, (2 * dim,), home),
+        _want("freq", freq, torch.float64, None, home), _on_device("k_cache", k_cache, dtype, home),
+        _on_device("v_cache", v_cache, dtype, home),
+        _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home),
+        _want("tree_sizes", tree_sizes, torch.int32, (batch,), home),
+        _want("depth", depth, torch.int32, (batch, tokens), home), table,
+        _want("status", status, torch.int32, None, home), _stream(stream, home))), "gqa_rope_append")
 
 
 def tree_workspace(batch: int, tokens: int, num_q_heads: int, num_kv_heads: int, device,
@@ -1046,41 +1063,31 @@ def tree_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, o
     their mask rows name (tree_masks(), on the device; None: a causal run) into `out` (packed)."""
     home = torch.cuda.current_device()
     batch, tokens, hq, dim = q.shape
-    p = _TreeDecodeParams()
-    p.dtype, p.batch, p.tokens = _dtype_code(q), batch, tokens
-    p.num_q_heads, p.num_kv_heads, p.head_dim = hq, num_kv_heads, dim
-    p.fixed_block = fixed_block
-    p.layout = layout.c()
-    p.q, p.q_token_stride = _token_rows("q", q, q.dtype, home)
-    p.k_cache, p.v_cache = _cache_pair(k_cache, v_cache, q.dtype, home)
-    p.out = _want("out", out, q.dtype, (batch, tokens, hq, dim), home)
-    p.mask_dev = _want("mask", mask, torch.int32, (batch, tokens, (tokens + 31) // 32), home)
-    p.seq_lens_dev = _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home)
-    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
-    if block_table is not None:
-        p.blocks_per_seq = block_table.shape[1]
-        p.block_table_dev = _want("block_table", block_table, torch.int32,
-                                  (batch, block_table.shape[1]), home)
-    if workspace is not None:
-        p.workspace = _want("workspace", workspace, torch.uint8, None, home)
-        p.workspace_bytes = workspace.numel()
-    p.status_dev = _want("status", status, torch.int32, None, home)
-    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
-    _check(lib().gqa_tree_decode(C.byref(p)), "gqa_tree_decode")
+    dtype = q.dtype
+    q_ptr, q_stride = _token_rows("q", q, dtype, home)
+    table, per_seq = _table(block_table, batch, home)
+    _check(lib().gqa_tree_decode(_TREE_DECODE.pack(
+        _dtype_code(q), batch, tokens, hq, num_kv_heads, dim, per_seq, fixed_block, layout.block_tokens,
+        layout.num_blocks, layout.stride_block, layout.stride_token, layout.stride_head, q_stride, q_ptr,
+        _on_device("k_cache", k_cache, dtype, home), _on_device("v_cache", v_cache, dtype, home),
+        _want("out", out, dtype, (batch, tokens, hq, dim), home),
+        _want("mask", mask, torch.int32, (batch, tokens, (tokens + 31) // 32), home),
+        _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home),
+        _want("tree_sizes", tree_sizes, torch.int32, (batch,), home), table,
+        _want("workspace", workspace, torch.uint8, None, home),
+        0 if workspace is None else workspace.numel(),
+        _want("status", status, torch.int32, None, home), _stream(stream, home))), "gqa_tree_decode")
 
 
 def _prob_rows(name: str, t: torch.Tensor, dtype, shape, home: int):
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {shape}")
-    if t.get_device() != home:
-        raise ValueError(f"{name}: on {t.device}, the current device is cuda:{home}")
-    if t.stride(2) != 1 and shape[2] != 1:
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != home:
+        _refuse(name, t, dtype, shape, home)
+    seq, node, word = t.stride()
+    if word != 1 and shape[2] != 1:
         raise ValueError(f"{name}: the vocabulary must be packed")
-    if (t.stride(0) == 0 and shape[0] > 1) or (t.stride(1) == 0 and shape[1] > 1):
+    if (seq == 0 and shape[0] > 1) or (node == 0 and shape[1] > 1):
         raise ValueError(f"{name}: rows that share memory (expanded) are not supported")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    return t.data_ptr(), seq, node
 
 
 def tree_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor,
@@ -1092,25 +1099,19 @@ def tree_verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: tor
     (row n: after node n) with the draft's probabilities (or None: drafts that were not sampled)
     and uniform numbers in [0, 1); leaves the accepted path, its length and the next token."""
     home = torch.cuda.current_device()
-    batch, nodes, vocab = target.shape
-    p = _TreeVerifyParams()
-    p.dtype, p.batch, p.tokens, p.vocab = _dtype_code(target), batch, nodes, vocab
-    p.target, p.target_seq_stride, p.target_node_stride = _prob_rows(
-        "target", target, target.dtype, (batch, nodes, vocab), home)
-    if draft is not None:
-        p.draft, p.draft_seq_stride, p.draft_node_stride = _prob_rows(
-            "draft", draft, target.dtype, (batch, nodes, vocab), home)
-    p.tokens_dev = _want("tokens", tokens, torch.int32, (batch, nodes), home)
-    p.parents_dev = _want("parents", parents, torch.int32, (batch, nodes), home)
-    p.u_accept = _want("u_accept", u_accept, torch.float32, (batch, nodes), home)
-    p.u_sample = _want("u_sample", u_sample, torch.float32, (batch,), home)
-    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
-    p.path = _want("path", path, torch.int32, (batch, nodes), home)
-    p.kept = _want("kept", kept, torch.int32, (batch,), home)
-    p.next_token = _want("next_token", next_token, torch.int32, (batch,), home)
-    p.status_dev = _want("status", status, torch.int32, None, home)
-    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
-    _check(lib().gqa_tree_verify(C.byref(p)), "gqa_tree_verify")
+    shape = batch, nodes, vocab = tuple(target.shape)
+    dtype = target.dtype
+    p_ptr, p_seq, p_node = _prob_rows("target", target, dtype, shape, home)
+    q_ptr, q_seq, q_node = (0, 0, 0) if draft is None else _prob_rows("draft", draft, dtype, shape, home)
+    each, one = (batch, nodes), (batch,)
+    _check(lib().gqa_tree_verify(_TREE_VERIFY.pack(
+        _dtype_code(target), batch, nodes, vocab, p_seq, p_node, q_seq, q_node, p_ptr, q_ptr,
+        _want("tokens", tokens, torch.int32, each, home), _want("parents", parents, torch.int32, each, home),
+        _want("u_accept", u_accept, torch.float32, each, home),
+        _want("u_sample", u_sample, torch.float32, one, home),
+        _want("tree_sizes", tree_sizes, torch.int32, one, home), _want("path", path, torch.int32, each, home),
+        _want("kept", kept, torch.int32, one, home), _want("next_token", next_token, torch.int32, one, home),
+        _want("status", status, torch.int32, None, home), _stream(stream, home))), "gqa_tree_verify")
 
 
 def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: int,
@@ -1124,22 +1125,15 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: i
     and leaves the new lengths in seq_lens_out (another tensor than seq_lens_dev)."""
     home = torch.cuda.current_device()
     batch, nodes = path.shape
-    p = _TreeCommitParams()
-    p.dtype, p.batch, p.tokens = _dtype_code(k_cache), batch, nodes
-    p.num_kv_heads, p.head_dim, p.num_layers = num_kv_heads, 128, layers
-    p.fixed_block = fixed_block
-    p.layout = layout.c()
-    p.layer_stride = k_cache.numel() // layers if layer_stride is None else layer_stride
-    p.k_cache, p.v_cache = _cache_pair(k_cache, v_cache, k_cache.dtype, home)
-    p.path = _want("path", path, torch.int32, (batch, nodes), home)
-    p.kept = _want("kept", kept, torch.int32, (batch,), home)
-    p.seq_lens_dev = _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home)
-    p.seq_lens_out = _want("seq_lens_out", seq_lens_out, torch.int32, (batch,), home)
-    p.tree_sizes_dev = _want("tree_sizes", tree_sizes, torch.int32, (batch,), home)
-    if block_table is not None:
-        p.blocks_per_seq = block_table.shape[1]
-        p.block_table_dev = _want("block_table", block_table, torch.int32,
-                                  (batch, block_table.shape[1]), home)
-    p.status_dev = _want("status", status, torch.int32, None, home)
-    p.stream = torch.cuda.current_stream().cuda_stream if stream is None else stream
-    _check(lib().gqa_tree_commit(C.byref(p)), "gqa_tree_commit")
+    dtype = k_cache.dtype
+    table, per_seq = _table(block_table, batch, home)
+    _check(lib().gqa_tree_commit(_TREE_COMMIT.pack(
+        _dtype_code(k_cache), batch, nodes, num_kv_heads, 128, layers, per_seq, fixed_block,
+        layout.block_tokens, layout.num_blocks, layout.stride_block, layout.stride_token, layout.stride_head,
+        k_cache.numel() // layers if layer_stride is None else layer_stride,
+        _on_device("k_cache", k_cache, dtype, home), _on_device("v_cache", v_cache, dtype, home),
+        _want("path", path, torch.int32, (batch, nodes), home), _want("kept", kept, torch.int32, (batch,), home),
+        _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home),
+        _want("tree_sizes", tree_sizes, torch.int32, (batch,), home), table,
+        _want("seq_lens_out", seq_lens_out, torch.int32, (batch,), home),
+        _want("status", status, torch.int32, None, home), _stream(stream, home))), "gqa_tree_commit")

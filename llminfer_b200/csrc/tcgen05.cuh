@@ -30,32 +30,35 @@ __device__ __forceinline__ void tc_fence_after() {
 // K-major operand (a row holds consecutive k): sbo = bytes between groups of 8 rows, lbo unused.
 // MN-major operand (a row holds 64 consecutive m or n of one k): sbo = bytes between groups of 8 k,
 // lbo = bytes between chunks of 64 m or n.
-__device__ __forceinline__ uint64_t smem_matrix(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lbo >> 4) << 16 |
-           (uint64_t)(sbo >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// The low word holds address and lbo and moves by bytes / 16 with the address; the high word is fixed.
+__device__ __forceinline__ uint32_t matrix_lo(uint32_t addr, uint32_t lbo) {
+    return (addr & 0x3ffffu) >> 4 | (lbo >> 4) << 16;
 }
+__host__ __device__ constexpr uint32_t matrix_hi(uint32_t sbo) { return sbo >> 4 | 1u << 14 | 2u << 29; }
 // BF16 operands, FP32 accumulator, M x N; b_mn: B is MN-major.
 __host__ __device__ constexpr uint32_t mma_shape(uint32_t m, uint32_t n, bool b_mn) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (b_mn ? 1u << 16 : 0u) | (n >> 3) << 17 | (m >> 4) << 24;
 }
 
 // ---- products (one thread) ------------------------------------------------------------------------
-// D[tmem] (+)= A[smem] B[smem], k = 16.
-__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape,
+// D[tmem] (+)= A[smem] B[smem], k = 16; `hi`: high word of both descriptors.
+__device__ __forceinline__ void tc_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t shape,
                                           bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(shape), "r"((uint32_t)accumulate)
         : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem], k = 16.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape,
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t hi, uint32_t shape,
                                           bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "mov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(hi), "r"(shape), "r"((uint32_t)accumulate)
         : "memory");
 }
 // Arrives on `bar` when all products this thread issued so far are complete.

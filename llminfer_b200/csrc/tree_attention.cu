@@ -13,7 +13,8 @@
 // share every key tile. While one stream computes weights, the tensor cores work for the other:
 //   S(j) .. weights(j) .. O += P(j) V, then S(j + 2) of the same stream, whose S and P share columns.
 // Warps 0-7: softmax, warp 8: bulk copies of Q, K and V into 128-byte swizzled rows (a ring of 32 KiB
-// tiles), warp 9: its lane 0 issues the products.
+// tiles), warp 9: its lane 0 issues the products (warps 10 and 11 only complete the warpgroup whose registers
+// the softmax warps take over).
 //
 // Work. All units (sequence, KV head, run of tokens) put their key tiles in one flat sequence that is cut evenly
 // over one CTA per SM, whatever the lengths are: few rows over a long history fill the GPU as well as
@@ -41,7 +42,8 @@ constexpr int kTileBytes = kTile * kHeadDim * 2;
 constexpr int kHalfBytes = kTileBytes / 2;      // 64 channels
 constexpr int kSlots = 6;                       // query tiles and ring together
 constexpr int kSoftmaxThreads = 256;
-constexpr int kThreads = kSoftmaxThreads + 64;
+constexpr int kThreads = kSoftmaxThreads + 128;
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;  // 256 * 224 + 128 * 56 = 384 * 168, what a launch gets
 constexpr int kUnitPad = 1;                     // places a unit counts on top of its tiles
 constexpr float kLazyMax = 8.0f;                // log2 of how far a score may exceed m
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -137,13 +139,26 @@ __device__ void build_tables(const TreeArgs& a, const Tables& t) {
     __syncthreads();
 }
 
-// CTAs that take part (none without a place), first place of CTA c, CTA that holds a place.
-__device__ __forceinline__ int used_ctas(const TreeArgs& a, int total) { return min(a.ctas, total); }
-__device__ __forceinline__ int cut_at(int c, int total, int ctas) {
-    return (int)((int64_t)min(c, ctas) * total / max(ctas, 1));
-}
-__device__ __forceinline__ int owner_of(int place, int total, int ctas) {
-    return (int)((((int64_t)place + 1) * ctas - 1) / total);
+// The places cut over the CTAs: the first `extra` take per + 1 places, the others per; none without a
+// place takes part. 32-bit arithmetic: every role does this before its first instruction of use.
+struct Cut {
+    int total;
+    int ctas;
+    int per;
+    int extra;
+    __device__ int begin(int c) const { return c >= ctas ? total : c * per + min(c, extra); }
+    __device__ int owner(int place) const {
+        const int wide = extra * (per + 1);
+        return place < wide ? place / (per + 1) : extra + (place - wide) / per;
+    }
+};
+__device__ __forceinline__ Cut cut_of(const TreeArgs& a, const Tables& t) {
+    Cut c;
+    c.total = t.base[a.batch];
+    c.ctas = min(a.ctas, c.total);
+    c.per = c.ctas > 0 ? c.total / c.ctas : 0;
+    c.extra = c.total - c.per * c.ctas;
+    return c;
 }
 
 struct Unit {
@@ -216,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                           const __grid_constant__ CUtensorMap map_v, const TreeArgs a) {
     constexpr int kRing = kSlots - QT;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t s_kv_full[kRing], s_kv_empty[kRing], s_q_full[QT], s_q_empty[QT];
+    __shared__ uint64_t s_kv_full[kRing], s_kv_empty[kRing], s_q_full[2], s_q_empty[2];
     __shared__ uint64_t s_s_full[2], s_p_ready[2], s_o_full[2], s_o_free[2], s_drain;
     __shared__ float s_ml[2][2][kTile];       // m (scaled, log2) and l of the streams' rows
     __shared__ uint32_t s_bad[2][4];          // nodes with a non-finite V row, by turns of the pieces
@@ -224,7 +239,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ int s_dead;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                ~static_cast<uintptr_t>(1023));
+    // Query tiles take their rows only (products read 128 rows: the others are never looked at), so that
+    // up to 64 rows leave room for the next piece's tile beside the current one.
     const uint32_t q_tiles = smem_u32(smem);
+    const uint32_t q_half = a.tile_rows * 128u;
+    const uint32_t q_slots = QT * kTileBytes >= 4 * (int)q_half ? 2 : 1;
     uint8_t* ring_ptr = smem + QT * kTileBytes;
     const uint32_t ring = smem_u32(ring_ptr);
     const Tables tables = tables_at(reinterpret_cast<int32_t*>(smem + kSlots * kTileBytes), a.batch);
@@ -236,7 +255,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(smem_u32(&s_kv_full[i]), 1);
             mbar_init(smem_u32(&s_kv_empty[i]), 1);
         }
-        for (int i = 0; i < QT; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&s_q_full[i]), 1);
             mbar_init(smem_u32(&s_q_empty[i]), 1);
         }
@@ -257,22 +276,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&map_v);
     }
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), kColumns);
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();
     build_tables<QT>(a, tables);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    const int total = tables.base[a.batch];
-    const int ctas = used_ctas(a, total);
-    int pos = cut_at(blockIdx.x, total, ctas);
-    const int pos_end = cut_at(blockIdx.x + 1, total, ctas);
+    const Cut cut = cut_of(a, tables);
+    int pos = cut.begin(blockIdx.x);
+    const int pos_end = cut.begin(blockIdx.x + 1);
     // One query tile: the streams take key tiles in turn; two: both take every key tile.
     auto two_tiles = [&](const Unit& u) { return QT == 2 && u.tokens > a.tile_tokens; };
 
-    if (warp == 8) {
+    if (warp >= 8) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      if (warp == 8) {
         // ---- bulk copies ---------------------------------------------------------------------------
         const uint64_t policy = l2_policy_evict_first();
         const int boxes = kTile / a.box_keys;
@@ -282,27 +302,27 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         while (ok && next_piece<QT>(a, tables, &pos, pos_end, &p)) {
             const bool two = two_tiles(p.u);
-            for (int st = 0; st < (two ? 2 : 1); ++st, ++q_fills) {
-                const uint32_t slot = q_fills % QT, round = q_fills / QT;
-                if (round > 0 && !wait_warp(smem_u32(&s_q_empty[slot]), (round - 1) & 1u, dead)) {
-                    ok = false;
-                    break;
-                }
-                if (lane == 0) {
-                    const uint32_t bar = smem_u32(&s_q_full[slot]);
-                    const int row = p.u.b * a.cache.tokens + p.u.token0 + st * a.tile_tokens;
-                    mbar_arrive_expect_tx(bar, q_bytes);
-                    for (int h = 0; h < 2; ++h) {
+            auto load_q = [&]() {
+                for (int st = 0; st < (two ? 2 : 1) && ok; ++st) {
+                    const uint32_t slot = q_fills % q_slots, round = q_fills / q_slots;
+                    if (round > 0 && !wait_warp(smem_u32(&s_q_empty[slot]), (round - 1) & 1u, dead)) ok = false;
+                    if (!ok) return;
+                    ++q_fills;
+                    if (lane < 2) {
+                        const uint32_t bar = smem_u32(&s_q_full[slot]);
+                        const int row = p.u.b * a.cache.tokens + p.u.token0 + st * a.tile_tokens;
+                        if (lane == 0) mbar_arrive_expect_tx(bar, q_bytes);
+                        __syncwarp(3u);
                         asm volatile(
                             "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
                             " [%0], [%1, {%3, %4, %5}], [%2];"
-                            ::"r"(q_tiles + slot * kTileBytes + h * kHalfBytes),
-                            "l"(reinterpret_cast<uint64_t>(&map_q)), "r"(bar), "r"(h * 64),
-                            "r"(p.u.hk * a.group), "r"(row)
+                            ::"r"(q_tiles + (2 * slot + lane) * q_half), "l"(reinterpret_cast<uint64_t>(&map_q)),
+                            "r"(bar), "r"(lane * 64), "r"(p.u.hk * a.group), "r"(row)
                             : "memory");
                     }
+                    __syncwarp();
                 }
-            }
+            };
             auto load = [&](const CUtensorMap* map, int t) {
                 const uint32_t slot = fills % kRing, round = fills / kRing;
                 if (round > 0 && !wait_warp(smem_u32(&s_kv_empty[slot]), (round - 1) & 1u, dead)) ok = false;
@@ -334,11 +354,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
             };
+            // The query tile goes first if its slot is free, else behind a ring full of keys and values: their
+            // copies run while the products of the last piece still read its queries.
             const int lead = min(two ? 1 : 2, p.tiles);
-            for (int t = 0; t < lead && ok; ++t) load(&map_k, t);
-            for (int t = 0; t < p.tiles && ok; ++t) {
-                load(&map_v, t);
-                if (t + lead < p.tiles) load(&map_k, t + lead);
+            int kt = 0, vt = 0;
+            const int q_at = q_fills + (two ? 2 : 1) <= q_slots ? 0 : min(kRing, 2 * p.tiles - 1);
+            for (int i = 0; i < 2 * p.tiles && ok; ++i) {
+                if (i == q_at) load_q();
+                if (kt < min(vt + lead, p.tiles)) {
+                    load(&map_k, kt++);
+                } else {
+                    load(&map_v, vt++);
+                }
             }
         }
         if (!ok) {
@@ -348,13 +375,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t f = fills > (uint32_t)kRing ? fills - kRing : 0; f < fills; ++f) {
                     wait_bar(smem_u32(&s_kv_full[f % kRing]), (f / kRing) & 1u, &fresh);
                 }
-                for (uint32_t f = q_fills > (uint32_t)QT ? q_fills - QT : 0; f < q_fills; ++f) {
-                    wait_bar(smem_u32(&s_q_full[f % QT]), (f / QT) & 1u, &fresh);
+                for (uint32_t f = q_fills > q_slots ? q_fills - q_slots : 0; f < q_fills; ++f) {
+                    wait_bar(smem_u32(&s_q_full[f % q_slots]), (f / q_slots) & 1u, &fresh);
                 }
             }
             __syncwarp();
         }
-    } else if (warp == 9) {
+      } else if (warp == 9) {
         // ---- products ------------------------------------------------------------------------------
         if (lane == 0) {
             constexpr uint32_t kShapeS = mma_shape(kTile, kTile, false);
@@ -369,25 +396,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Order order = {p.tiles, two ? 1 : 2};
                 for (int st = 0; st < (two ? 2 : 1) && ok; ++st) {
                     const uint32_t f = q_pos + st;
-                    ok = wait_bar(smem_u32(&s_q_full[f % QT]), (f / QT) & 1u, dead);
+                    ok = wait_bar(smem_u32(&s_q_full[f % q_slots]), (f / q_slots) & 1u, dead);
                 }
                 auto issue_s = [&](int j) {
                     const int st = j & 1, t = two ? j >> 1 : j;
                     const uint32_t f = ring_pos + order.k(t), slot = f % kRing;
                     ok = ok && wait_bar(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
                     if (!ok) return;
-                    const uint32_t q = q_tiles + ((q_pos + (two ? st : 0)) % QT) * kTileBytes;
-                    const uint32_t k = ring + slot * kTileBytes;
+                    const uint32_t q = matrix_lo(q_tiles + ((q_pos + (two ? st : 0)) % q_slots) * 2 * q_half, 16);
+                    const uint32_t k = matrix_lo(ring + slot * kTileBytes, 16);
 #pragma unroll
                     for (int i = 0; i < kHeadDim / 16; ++i) {
-                        const uint32_t off = (i >> 2) * kHalfBytes + (i & 3) * 32;
-                        tc_mma_ss(tmem + kColS + st * 128, smem_matrix(q + off, 16, 1024),
-                                  smem_matrix(k + off, 16, 1024), kShapeS, i > 0);
+                        tc_mma_ss(tmem + kColS + st * 128, q + (i >> 2) * (q_half >> 4) + (i & 3) * 2,
+                                  k + (i >> 2) * (kHalfBytes >> 4) + (i & 3) * 2, matrix_hi(1024), kShapeS, i > 0);
                     }
                     tc_commit(smem_u32(&s_s_full[st]));
                     if (!two || st == 1) tc_commit(smem_u32(&s_kv_empty[slot]));
                     if (j == count - 1) {
-                        for (int i = 0; i < (two ? 2 : 1); ++i) tc_commit(smem_u32(&s_q_empty[(q_pos + i) % QT]));
+                        for (int i = 0; i < (two ? 2 : 1); ++i) tc_commit(smem_u32(&s_q_empty[(q_pos + i) % q_slots]));
                     }
                 };
                 issue_s(0);
@@ -403,11 +429,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t v = ring + slot * kTileBytes;
+                    const uint32_t v = matrix_lo(ring + slot * kTileBytes, kHalfBytes);
 #pragma unroll
                     for (int i = 0; i < kTile / 16; ++i) {
-                        tc_mma_ts(tmem + kColO + st * 128, tmem + kColS + st * 128 + i * 8,
-                                  smem_matrix(v + i * 2048, kHalfBytes, 1024), kShapeO, j >= 2 || i > 0);
+                        tc_mma_ts(tmem + kColO + st * 128, tmem + kColS + st * 128 + i * 8, v + i * (2048 >> 4),
+                                  matrix_hi(1024), kShapeO, j >= 2 || i > 0);
                     }
                     if (!two || st == 1) tc_commit(smem_u32(&s_kv_empty[slot]));
                     if (j + 2 >= count) {
@@ -428,7 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
+      }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ---- weights ---------------------------------------------------------------------------------
         const int st = warp >> 2;             // stream
         const int row = threadIdx.x & 127;    // of the stream's query tile; lane of tensor memory
@@ -438,8 +466,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int words = (a.cache.tokens + 31) / 32;
         uint32_t ring_pos = 0, jobs = 0, pieces[2] = {0, 0}, turn = 0;
         bool ok = true;
+        int last_cta = -1;  // of the unit this CTA starts and others finish
         Piece p;
         while (ok && next_piece<QT>(a, tables, &pos, pos_end, &p)) {
+            if (threadIdx.x == 0 && !p.whole && p.tile == 0) {
+                last_cta = cut.owner(p.u.place + kUnitPad + p.u.tiles - 1);
+                a.cut_units[2 * blockIdx.x] = make_int4(last_cta, p.u.b, p.u.hk, p.u.token0);
+                a.cut_units[2 * blockIdx.x + 1] = make_int4(p.u.tokens, 0, 0, 0);
+            }
             const bool two = two_tiles(p.u);
             const int count = two ? 2 * p.tiles : p.tiles;
             const Order order = {p.tiles, two ? 1 : 2};
@@ -680,6 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (active1) ++pieces[1];
             ++turn;
         }
+        if (threadIdx.x == 0 && last_cta < 0) a.cut_units[2 * blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
     __syncthreads();
     if (s_dead && threadIdx.x == 0 && a.cache.status != nullptr) atomicExch(a.cache.status, kStatusStageTimeout);
@@ -690,40 +725,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Merges the records of the units that were cut: out = sum_i O_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), pieces in
-// ascending order. grid.x: units, or (by_cut) the cuts between CTAs, of which the first inside a unit
-// stands for it; grid.y: groups of 8 rows. Thread: row tid % 8 of the group, channels 4 (tid / 8) .. + 3.
+// ascending order. grid.x: CTAs of the launch before, each of which starts at most one unit that others
+// finish and has left its description; grid.y: groups of 8 rows. Thread: row tid % 8 of the group, channels
+// 4 (tid / 8) .. + 3.
 template <int QT>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int by_cut) {
-    extern __shared__ int32_t s_tables[];
-    const Tables t = tables_at(s_tables, a.batch);
+__global__ void __launch_bounds__(256, 4) tree_merge_kernel(const TreeArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    build_tables<QT>(a, t);
-    const int total = t.base[a.batch];
-    const int ctas = used_ctas(a, total);
-    Unit u;
-    if (by_cut) {
-        const int c = blockIdx.x + 1;
-        if (c >= ctas) return;
-        const int at = cut_at(c, total, ctas);
-        u = unit_at<QT>(a, t, at);
-        const int first = u.place + kUnitPad;
-        if (at <= first || cut_at(c - 1, total, ctas) > first) return;
-    } else {
-        // The blockIdx.x-th unit: the sequences' units in order.
-        int b = 0, i = blockIdx.x;
-        while (b < a.batch) {
-            const int here = t.n[b] > 0 ? units_of<QT>(a, t.n[b]) : 0;
-            if (i < here) break;
-            i -= here;
-            ++b;
-        }
-        if (b == a.batch) return;
-        u = unit_at<QT>(a, t, t.base[b] + i * places_of(t.len[b]));
-    }
-    const int lo = u.place + kUnitPad;
-    const int c0 = owner_of(lo, total, ctas), c1 = owner_of(lo + u.tiles - 1, total, ctas);
-    if (c0 == c1) return;  // whole: already written
+    const int4 head = __ldcg(a.cut_units + 2 * blockIdx.x);
+    const int c0 = blockIdx.x, c1 = head.x;
+    if (c1 < 0) return;
+    struct {
+        int b, hk, token0, tokens;
+    } u = {head.y, head.z, head.w, __ldcg(a.cut_units + 2 * blockIdx.x + 1).x};
     const int tiles_rows = a.tile_tokens * a.group;
     const int r = blockIdx.y * 8 + (threadIdx.x & 7);  // row of the unit
     if (r >= u.tokens * a.group) return;
@@ -734,7 +748,7 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int b
     auto at = [&](int c) { return rec + (int64_t)(2 * c + (c == c0 ? 1 : 0)) * record; };
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    constexpr int kBatch = 8;
+    constexpr int kBatch = 6;
     for (int c = c0; c <= c1; c += kBatch) {
         float mi[kBatch], li[kBatch];
         float4 oi[kBatch];
@@ -743,9 +757,9 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeArgs a, int b
             mi[i] = -INFINITY;
             if (c + i > c1) continue;
             const float* p = at(c + i);
-            mi[i] = p[kHeadDim * a.tile_rows + row];
-            li[i] = p[(kHeadDim + 1) * a.tile_rows + row];
-            oi[i] = *reinterpret_cast<const float4*>(p + ((int64_t)chunk * a.tile_rows + row) * 4);
+            mi[i] = __ldcg(p + kHeadDim * a.tile_rows + row);
+            li[i] = __ldcg(p + (kHeadDim + 1) * a.tile_rows + row);
+            oi[i] = __ldcg(reinterpret_cast<const float4*>(p + ((int64_t)chunk * a.tile_rows + row) * 4));
         }
         float next = m;
 #pragma unroll
@@ -799,24 +813,26 @@ int launch(const TreeArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, cons
     if (launch_pdl(kernel, dim3(a.ctas), dim3(kThreads), smem, stream, mq, mk, mv, a) != cudaSuccess) {
         return GQA_ERR_CUDA;
     }
-    const int64_t units = (int64_t)a.batch * a.num_kv_heads * ceil_div(a.cache.tokens, a.tile_tokens * QT);
-    const int by_cut = units > a.ctas ? 1 : 0;
     const int unit_tokens = a.cache.tokens < a.tile_tokens * QT ? a.cache.tokens : a.tile_tokens * QT;
-    const dim3 grid((unsigned)(by_cut ? a.ctas - 1 : units), (unsigned)ceil_div(unit_tokens * a.group, 8));
-    if (by_cut && a.ctas < 2) return GQA_OK;
-    return launch_pdl(tree_merge_kernel<QT>, grid, dim3(256), table_bytes(a.batch), stream, a, by_cut) == cudaSuccess
-               ? GQA_OK
-               : GQA_ERR_CUDA;
+    const dim3 grid((unsigned)a.ctas, (unsigned)ceil_div(unit_tokens * a.group, 8));
+    return launch_pdl(tree_merge_kernel<QT>, grid, dim3(256), 0, stream, a) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
 }  // namespace
 
-size_t tree_attention_workspace(int32_t tokens, int32_t group, int32_t ctas) {
+// Records, then the descriptions of the cut units.
+static size_t record_bytes(int32_t tokens, int32_t group, int32_t ctas) {
     return (size_t)2 * ctas * query_tiles(tokens, group) * rows_per_tile(tokens, group) * kRecordCols * sizeof(float);
+}
+
+size_t tree_attention_workspace(int32_t tokens, int32_t group, int32_t ctas) {
+    return record_bytes(tokens, group, ctas) + 2 * (size_t)ctas * sizeof(int4);
 }
 
 int launch_tree_attention(TreeArgs a, const gqa_kv_layout& layout, int32_t sm_count, cudaStream_t stream) {
     a.ctas = sm_count;
+    a.cut_units = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(a.workspace) +
+                                          record_bytes(a.cache.tokens, a.group, sm_count));
     a.tile_tokens = kTile / a.group;
     a.tile_rows = rows_per_tile(a.cache.tokens, a.group);
     a.box_tokens = a.cache.tokens < a.tile_tokens ? a.cache.tokens : a.tile_tokens;

@@ -13,6 +13,7 @@ struct TreeArgs {
     void* out;
     const uint32_t* mask;  // [batch][tokens][words] or null: a causal run
     float* workspace;      // partial records (BF16 path)
+    int4* cut_units;       // [ctas][2], behind the records: the unit a CTA starts and does not finish
     int64_t q_stride;      // elements between tokens of q
     int32_t batch;
     int32_t num_q_heads;

@@ -8,11 +8,16 @@
 // the walk starts. Tests and sums are FP64: p, q and u are FP32 or BF16 values, so u q is exact and the
 // outcome does not depend on how the sum was cut.
 //
+// Without draft probabilities the residual is p without the rejected tokens. One pass per node then
+// serves all its children: R = the sum of p without any child's token; after j rejections the
+// sum is R plus p at the tokens still to be tried (only positive terms: nothing cancels).
+//
 // One thread-block cluster per sequence; the CTAs take equal slices of the vocabulary, the warps of
 // a CTA contiguous segments of its slice. Every CTA walks the tree itself (same inputs, same sums,
 // same steps); after a pass the CTAs read one another's partial sums through distributed shared
 // memory. To place the sample, the partial sums name the segment in which the cumulative sum
-// passes u S, and one warp walks that segment again.
+// passes u S, and one warp walks that segment again. A pass is bound by the latency of its loads: a lane
+// has four vectors in flight.
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -51,13 +56,12 @@ __device__ __forceinline__ float value(const float* p) { return __ldg(p); }
 __device__ __forceinline__ float value(const __nv_bfloat16* p) {
     return __uint_as_float((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p)) << 16);
 }
-// 16 bytes of a row.
-__device__ __forceinline__ void vector_of(const float* p, float (&x)[4]) {
-    const float4 u = __ldg(reinterpret_cast<const float4*>(p));
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+// 16 bytes of a row as its elements.
+__device__ __forceinline__ void elements(uint4 u, float (&x)[4]) {
+    x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y);
+    x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
 }
-__device__ __forceinline__ void vector_of(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void elements(uint4 u, float (&x)[8]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -66,19 +70,31 @@ __device__ __forceinline__ void vector_of(const __nv_bfloat16* p, float (&x)[8])
     }
 }
 
-// max(p - c q, 0); NaN and negative entries count as 0, and q counts as 0 where it is no number.
+// An FP32 number as FP64, by its bits: the conversion instruction runs at a quarter of the rate of FP64
+// arithmetic and would bound a pass. Negative numbers, NaN and numbers below 2^-126 give 0, infinity 2^128.
+__device__ __forceinline__ double widen(float x) {
+    const uint32_t u = __float_as_uint(fmaxf(x, 0.0f));
+    const bool some = u >= 0x00800000u;
+    return __hiloint2double(some ? (int)((u >> 3) + 0x38000000u) : 0, some ? (int)(u << 29) : 0);
+}
+// max(p - c q, 0)
 __device__ __forceinline__ double rest_of(float p, float q, double c) {
-    return fmax(fma(-c, (double)fmaxf(q, 0.0f), (double)fmaxf(p, 0.0f)), 0.0);
+    const double r = fma(-c, widen(q), widen(p));
+    return __double2hiint(r) < 0 ? 0.0 : r;
 }
 
 // Where the walk stands.
+enum Action : int {
+    kSum,     // a pass over the current node's rows, then on with the walk
+    kSample,  // a pass, then the sample
+    kPlace,   // the sample from the sums of the last pass
+};
 struct Walk {
-    int node;       // current node
-    int tried;      // its last tried child (or the node itself)
-    int count;      // nodes on the path
-    int rejected;   // children of `node` rejected so far
-    int pass;       // 1: the sum of the residual is needed, 0: the walk has ended
-    int last;       // no child is left: the sum is for the sample
+    int node;      // current node
+    int tried;     // its last tried child (or the node itself)
+    int count;     // nodes on the path
+    int rejected;  // children of `node` rejected so far
+    int action;
     double c;
     double sum;
 };
@@ -98,13 +114,18 @@ __device__ __forceinline__ Said ld_cluster_said(uint32_t addr) {
 }
 
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyArgs a) {
     constexpr int VE = 16 / (int)sizeof(T);
+    constexpr int kUnroll = DRAFT ? 2 : 4;  // vectors of a row a lane has in flight
     __shared__ uint32_t s_child[kTreeMaxTokens][kWords];
     __shared__ float s_p[kTreeMaxTokens], s_q[kTreeMaxTokens], s_u[kTreeMaxTokens];
     __shared__ int32_t s_word[kTreeMaxTokens];
     __shared__ int32_t s_path[kTreeMaxTokens];
-    __shared__ int32_t s_gone[kTreeMaxTokens];  // rejected tokens (draft without probabilities)
+    __shared__ uint8_t s_again[kTreeMaxTokens];        // an earlier sibling has the same token
+    __shared__ double s_ahead[kTreeMaxTokens];         // p at the tokens of later siblings
+    __shared__ int32_t s_gone[kTreeMaxTokens];         // tokens left out of the sum (no draft)
+    __shared__ uint8_t s_hit[kWarps][kTreeMaxTokens];  // those inside a warp's segment
+    __shared__ int s_gone_count;
     __shared__ double s_warp[kWarps];
     __shared__ Said s_said[2];  // this CTA's sum and step, buffers in turn: read by the whole cluster
     __shared__ Walk w;
@@ -112,33 +133,55 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
     const int rank = blockIdx.x % a.cluster;
     const int b = blockIdx.x / a.cluster;
     pdl_launch_dependents();
+    for (int i = tid; i < kTreeMaxTokens * kWords; i += kThreads) (&s_child[0][0])[i] = 0;
+    if (tid == 0) {
+        w = Walk{0, 0, 1, 0, kSum, 0.0, 1.0};
+        s_gone_count = 0;
+    }
     pdl_wait();
-    int n = a.tree_sizes != nullptr ? __ldg(a.tree_sizes + b) : a.tokens;
-    bool bad = n < 0 || n > a.tokens;
-    if (bad) n = 0;
     const T* target = static_cast<const T*>(a.target) + b * a.target_seq;
     const T* draft = DRAFT ? static_cast<const T*>(a.draft) + b * a.draft_seq : nullptr;
 
     // ---- children and the values at the drafted tokens ----------------------------------------
-    for (int i = tid; i < kTreeMaxTokens * kWords; i += kThreads) (&s_child[0][0])[i] = 0;
-    __syncthreads();
-    if (tid > 0 && tid < n) {
-        const int par = __ldg(a.parents + (int64_t)b * a.tokens + tid);
-        const int word = __ldg(a.words + (int64_t)b * a.tokens + tid);
-        s_word[tid] = word;
-        s_u[tid] = __ldg(a.u_accept + (int64_t)b * a.tokens + tid);
-        if (par >= 0 && par < tid && word >= 0 && word < a.vocab) {
-            s_p[tid] = fmaxf(value(target + par * a.target_node + word), 0.0f);
-            s_q[tid] = DRAFT ? fmaxf(value(draft + par * a.draft_node + word), 0.0f) : 1.0f;
-            atomicOr(&s_child[par][tid >> 5], 1u << (tid & 31));
-        } else {
-            bad = true;
-        }
+    int par = -1, word = -1;
+    float u = 0.0f;
+    if (tid > 0 && tid < a.tokens) {
+        par = __ldg(a.parents + (int64_t)b * a.tokens + tid);
+        word = __ldg(a.words + (int64_t)b * a.tokens + tid);
+        u = __ldg(a.u_accept + (int64_t)b * a.tokens + tid);
     }
-    if (tid == 0) w = Walk{0, 0, 1, 0, 0, 0, 0.0, 1.0};
-    if (tid < kTreeMaxTokens) s_path[tid] = -1;
+    const float u_sample = __ldg(a.u_sample + b);
+    int n = a.tree_sizes != nullptr ? __ldg(a.tree_sizes + b) : a.tokens;
+    bool bad = n < 0 || n > a.tokens;
+    if (bad) n = 0;
+    const bool node = tid > 0 && tid < n;
+    const bool fine = node && par >= 0 && par < tid && word >= 0 && word < a.vocab;
+    bad = bad || (node && !fine);
+    __syncthreads();
+    if (fine) {
+        const float p = value(target + par * a.target_node + word);
+        const float q = DRAFT ? value(draft + par * a.draft_node + word) : 1.0f;
+        atomicOr(&s_child[par][tid >> 5], 1u << (tid & 31));
+        s_word[tid] = word;
+        s_u[tid] = u;
+        s_p[tid] = p;
+        s_q[tid] = q;
+    }
     bad = __syncthreads_or(bad);
     if (bad && rank == 0 && tid == 0) raise_bad_input(a.status);
+    if (!DRAFT) {
+        if (fine) {
+            bool again = false;
+            for (int k = 0; k < kWords; ++k) {
+                uint32_t bits = s_child[par][k];
+                if (k == (tid >> 5)) bits &= (1u << (tid & 31)) - 1u;
+                if (k > (tid >> 5)) bits = 0;
+                for (; bits != 0; bits &= bits - 1) again = again || s_word[k * 32 + __ffs(bits) - 1] == word;
+            }
+            s_again[tid] = again;
+        }
+        __syncthreads();
+    }
 
     const T* p_row = target;
     const T* q_row = draft;
@@ -147,28 +190,62 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
     double before = 0.0;     // of the CTAs before this one
     double own = 0.0;
     bool later = false;      // a CTA after this one has something in its slice
-    // This CTA's and warp's vectors of 16 bytes. A vector is cut at the row's ends, where single
-    // elements are read; rows p and q that are not equally aligned are read element by element.
-    int vec_lo = 0, vec_hi = 0, shift = 0;
+    double run_to = 0.0;     // lane i: sum of this CTA's segments 0 .. i
+    // The row in vectors of 16 bytes. A vector is cut at the row's ends, where single elements are
+    // read; rows p and q that are not equally aligned are read element by element.
+    int vecs = 0, shift = 0;
     bool wide = false;
 
-    auto set_rows = [&](int node) {
-        p_row = target + node * a.target_node;
-        if (DRAFT) q_row = draft + node * a.draft_node;
+    auto set_rows = [&](int at) {
+        p_row = target + at * a.target_node;
+        if (DRAFT) q_row = draft + at * a.draft_node;
         shift = (int)((reinterpret_cast<uintptr_t>(p_row) & 15u) / sizeof(T));
         wide = !DRAFT || ((reinterpret_cast<uintptr_t>(p_row) ^ reinterpret_cast<uintptr_t>(q_row)) & 15u) == 0;
-        const int64_t vecs = (a.vocab + shift + VE - 1) / VE;
-        const int64_t lo = vecs * rank / a.cluster, hi = vecs * (rank + 1) / a.cluster;
-        vec_lo = (int)(lo + (hi - lo) * warp / kWarps);
-        vec_hi = (int)(lo + (hi - lo) * (warp + 1) / kWarps);
+        vecs = (a.vocab + shift + VE - 1) / VE;
     };
-    // The residual at the elements of vector `vec`; elements outside the row are 0.
-    auto residual = [&](int vec, double c, int rejected, double (&r)[VE]) {
+    // First vector of segment `seg` of this CTA's slice.
+    auto segment = [&](int seg) -> int {
+        const int64_t lo = (int64_t)vecs * rank / a.cluster, hi = (int64_t)vecs * (rank + 1) / a.cluster;
+        return (int)(lo + (hi - lo) * seg / kWarps);
+    };
+    // The tokens left out that lie in vectors [first, end), into this warp's list.
+    auto collect = [&](int first, int end, int gone) -> int {
+        int hits = 0;
+        for (int k0 = 0; k0 < gone; k0 += 32) {
+            const int k = k0 + lane;
+            const int vec = k < gone ? (s_gone[k] + shift) / VE : -1;
+            const bool in = vec >= first && vec < end;
+            const uint32_t some = __ballot_sync(0xffffffffu, in);
+            if (in) s_hit[warp][hits + __popc(some & ((1u << lane) - 1u))] = (uint8_t)k;
+            hits += __popc(some);
+        }
+        __syncwarp();
+        return hits;
+    };
+    auto whole = [&](int vec) { return vec * VE >= shift && vec * VE - shift + VE <= a.vocab; };
+    // The residual of a vector from its elements; `hits` tokens are left out.
+    auto rest = [&](int vec, const float (&p)[VE], const float (&q)[VE], double c, int hits, double (&r)[VE]) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+            r[i] = DRAFT && c > 0.0 ? rest_of(p[i], q[i], c) : widen(p[i]);
+        }
+        if (!DRAFT) {
+            for (int k = 0; k < hits; ++k) {
+                const int at = s_gone[s_hit[warp][k]] + shift - vec * VE;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    if (at == i) r[i] = 0.0;
+                }
+            }
+        }
+    };
+    // The residual at any vector; elements outside the row are 0.
+    auto residual = [&](int vec, double c, int hits, double (&r)[VE]) {
         const int e0 = vec * VE - shift;
         float p[VE], q[VE];
-        if (wide && e0 >= 0 && e0 + VE <= a.vocab) {
-            vector_of(p_row + e0, p);
-            if (DRAFT && c > 0.0) vector_of(q_row + e0, q);
+        if (wide && whole(vec)) {
+            elements(__ldg(reinterpret_cast<const uint4*>(p_row + e0)), p);
+            if (DRAFT && c > 0.0) elements(__ldg(reinterpret_cast<const uint4*>(q_row + e0)), q);
         } else {
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
@@ -177,46 +254,19 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
                 if (DRAFT && c > 0.0) q[i] = in ? value(q_row + e0 + i) : 0.0f;
             }
         }
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            r[i] = DRAFT && c > 0.0 ? rest_of(p[i], q[i], c) : (double)fmaxf(p[i], 0.0f);
-        }
-        if (!DRAFT) {
-            for (int k = 0; k < rejected; ++k) {
-                const int at = s_gone[k] - e0;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    if (at == i) r[i] = 0.0;
-                }
-            }
-        }
+        rest(vec, p, q, c, hits, r);
     };
-    // The sum of the residual over the vocabulary, the same value in every thread of the cluster.
-    // False: the CTAs do not agree where the walk stands.
-    auto pass = [&](double c, int rejected) -> bool {
-        uint64_t lead = 0;
-        double sum = 0.0;
-        for (int vec = vec_lo + lane; vec < vec_hi; vec += 32) {
-            double r[VE];
-            residual(vec, c, rejected, r);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) sum += r[i];
-        }
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) s_warp[warp] = sum;
-        __syncthreads();
-        own = 0.0;
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) own += s_warp[i];
-        // Every CTA reads the sums in the same order: the running sums are the same in all of them.
-        const uint64_t step = (uint64_t)n | (uint64_t)w.node << 8 | (uint64_t)rejected << 16 |
-                              (uint64_t)w.last << 24 | (uint64_t)(uint32_t)turn << 32;
+    // The sums of the cluster's CTAs, the same values in every thread. False: the CTAs do not agree
+    // where the walk stands.
+    auto exchange = [&]() -> bool {
+        const uint64_t step = (uint64_t)n | (uint64_t)w.node << 8 | (uint64_t)w.rejected << 16 |
+                              (uint64_t)w.action << 24 | (uint64_t)(uint32_t)turn << 32;
         if (tid == 0) s_said[turn & 1] = Said{own, step};
         cluster_sync_all();
         total = before = 0.0;
         later = false;
         bool agreed = true;
+        uint64_t lead = 0;
         for (int k = 0; k < a.cluster; ++k) {
             const Said said = ld_cluster_said(cluster_map(smem_u32(&s_said[turn & 1]), (uint32_t)k));
             if (k == 0) lead = said.step;
@@ -228,117 +278,162 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
         ++turn;
         return agreed;
     };
+    auto pass = [&](double c, int gone) -> bool {
+        const int lo = segment(warp), hi = segment(warp + 1);
+        const int hits = DRAFT ? 0 : collect(lo, hi, gone);
+        double sum = 0.0;
+        for (int v0 = lo + lane; v0 < hi; v0 += 32 * kUnroll) {
+            // The ends of the row are cut off here and added below.
+            uint4 up[kUnroll], uq[kUnroll];
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                const int vec = v0 + 32 * k;
+                if (vec < hi && wide && whole(vec)) {
+                    up[k] = __ldg(reinterpret_cast<const uint4*>(p_row + (vec * VE - shift)));
+                    if (DRAFT && c > 0.0) uq[k] = __ldg(reinterpret_cast<const uint4*>(q_row + (vec * VE - shift)));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kUnroll; ++k) {
+                const int vec = v0 + 32 * k;
+                if (vec >= hi) continue;
+                double r[VE];
+                if (wide && whole(vec)) {
+                    float p[VE], q[VE];
+                    elements(up[k], p);
+                    if (DRAFT && c > 0.0) elements(uq[k], q);
+                    rest(vec, p, q, c, hits, r);
+                } else {
+                    residual(vec, c, hits, r);
+                }
+#pragma unroll
+                for (int i = 0; i < VE; ++i) sum += r[i];
+            }
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) s_warp[warp] = sum;
+        __syncthreads();
+        // The running sums of the segments, in lanes 0 .. kWarps - 1 of every warp.
+        run_to = lane < kWarps ? s_warp[lane] : 0.0;
+#pragma unroll
+        for (int d = 1; d < kWarps; d <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, run_to, d);
+            if (lane >= d) run_to += up;
+        }
+        own = __shfl_sync(0xffffffffu, run_to, kWarps - 1);
+        const bool agreed = exchange();
+        __syncthreads();
+        return agreed;
+    };
+    // The child of w.node after w.tried, -1: none.
+    auto next_child = [&]() -> int {
+        for (int k = w.tried >> 5; k < kWords; ++k) {
+            uint32_t bits = s_child[w.node][k];
+            if (k == (w.tried >> 5)) bits &= ~((2u << (w.tried & 31)) - 1u);
+            if (bits != 0) return k * 32 + __ffs(bits) - 1;
+        }
+        return -1;
+    };
 
     // ---- the walk ---------------------------------------------------------------------------------
+    bool agreed = true;
+    int gone = 0;
     for (;;) {
-        if (tid == 0 && n == 0) w.last = 1;  // nothing to walk: one pass over nothing
+        if (tid == 0 && n == 0) w.action = kPlace;  // nothing to walk
         if (tid == 0 && n > 0) {
             for (;;) {
-                int child = -1;
-                for (int k = w.tried >> 5; k < kWords && child < 0; ++k) {
-                    uint32_t bits = s_child[w.node][k];
-                    if (k == (w.tried >> 5)) bits &= ~((2u << (w.tried & 31)) - 1u);
-                    if (bits != 0) child = k * 32 + __ffs(bits) - 1;
-                }
+                const int child = next_child();
                 if (child < 0) {
-                    w.last = 1;
-                    w.pass = 1;
+                    w.action = !DRAFT && w.rejected > 0 ? kPlace : kSample;
                     break;
                 }
                 w.tried = child;
-                double room = rest_of(s_p[child], DRAFT && w.c > 0.0 ? s_q[child] : 0.0f, w.c);
-                if (!DRAFT) {
-                    for (int k = 0; k < w.rejected; ++k) {
-                        if (s_gone[k] == s_word[child]) room = 0.0;
-                    }
-                }
-                if ((double)s_u[child] * (double)s_q[child] * w.sum < room) {
+                const double room = DRAFT ? rest_of(s_p[child], w.c > 0.0 ? s_q[child] : 0.0f, w.c)
+                                          : s_again[child] ? 0.0 : widen(s_p[child]);
+                if ((double)s_u[child] * widen(s_q[child]) * w.sum < room) {
                     w.node = child;
                     w.c = 0.0;
                     w.sum = 1.0;
                     w.rejected = 0;
+                    s_gone_count = 0;
                     s_path[w.count++] = child;
-                } else {
+                    continue;
+                }
+                ++w.rejected;
+                if (DRAFT) {
                     w.c += w.sum;
-                    s_gone[w.rejected++] = s_word[child];
-                    // Is another child left? If not, the pass for this rejection is the sample's too.
-                    bool more = false;
-                    for (int k = w.tried >> 5; k < kWords; ++k) {
-                        uint32_t bits = s_child[w.node][k];
-                        if (k == (w.tried >> 5)) bits &= ~((2u << (w.tried & 31)) - 1u);
-                        more = more || bits != 0;
-                    }
-                    w.last = more ? 0 : 1;
-                    w.pass = 1;
+                    w.action = next_child() < 0 ? kSample : kSum;
                     break;
                 }
+                if (w.rejected > 1) {
+                    w.sum = total + s_ahead[child];
+                    continue;
+                }
+                // The first rejection here: all children's tokens leave the sum.
+                int count = 0;
+                double ahead = 0.0;
+                for (int k = kWords - 1; k >= 0; --k) {
+                    for (uint32_t bits = s_child[w.node][k]; bits != 0;) {
+                        const int at = k * 32 + 31 - __clz(bits);
+                        bits &= ~(1u << (at & 31));
+                        s_ahead[at] = ahead;
+                        if (!s_again[at]) {
+                            s_gone[count++] = s_word[at];
+                            ahead += widen(s_p[at]);
+                        }
+                    }
+                }
+                s_gone_count = count;
+                w.action = kSum;
+                break;
             }
         }
         __syncthreads();
+        const int action = w.action;
         const double c = w.c;
-        const int rejected = w.rejected;
-        const bool last = w.last != 0;
-        if (n > 0) set_rows(w.node);
-        bool agreed = pass(c, rejected);
-        __syncthreads();
-        if (agreed && !last) {
-            if (tid == 0) w.sum = total;
+        if (action == kPlace) {
+            agreed = exchange();
+            __syncthreads();
+        } else {
+            gone = s_gone_count;
+            set_rows(w.node);
+            agreed = pass(c, gone);
+        }
+        if (!agreed || n == 0) break;
+        if (action == kSum) {
+            if (tid == 0) w.sum = DRAFT ? total : total + s_ahead[w.tried];
             continue;
         }
         double cc = c;
-        int gone = rejected;
-        if (agreed && !(total > 0.0) && rejected > 0) {  // nothing is left of p: p itself
+        if (!(total > 0.0) && w.rejected > 0) {  // nothing is left of p: p itself
             cc = 0.0;
             gone = 0;
             agreed = pass(cc, gone);
-            __syncthreads();
-        }
-        if (!agreed || n == 0) {
-            if (rank == 0) {
-                if (!agreed && tid == 0) raise_bad_input(a.status);
-                if (tid < a.tokens) a.path[(int64_t)b * a.tokens + tid] = -1;
-                if (tid == 0) {
-                    a.kept[b] = 0;
-                    a.next_token[b] = -1;
-                }
-            }
-            break;
+            if (!agreed) break;
         }
         // ---- the sample -----------------------------------------------------------------------
         // The first CTA whose running sum passes the threshold (or the last one with anything in it)
         // holds the sample; in it, likewise, the warp, the round of 32 vectors, the lane.
-        const double threshold = (double)__ldg(a.u_sample + b) * total;
+        const double threshold = (double)u_sample * total;
         // The running sums are the same numbers in every CTA, so exactly one of them passes it.
         const bool mine = total > threshold ? !(before > threshold) && before + own > threshold
                                             : own > 0.0 && !later;
         if (mine && warp == 0) {
-            double run = before;
-            int seg = -1, fallback = 0;
-            double seg_run = run;
-            for (int i = 0; i < kWarps; ++i) {
-                if (s_warp[i] > 0.0) {
-                    fallback = i;
-                    seg_run = run;
-                    if (run + s_warp[i] > threshold) {
-                        seg = i;
-                        break;
-                    }
-                }
-                run += s_warp[i];
-            }
-            if (seg < 0) seg = fallback;
-            run = seg_run;
-            const int64_t vecs = (a.vocab + shift + VE - 1) / VE;
-            const int64_t lo = vecs * rank / a.cluster, hi = vecs * (rank + 1) / a.cluster;
-            const int first = (int)(lo + (hi - lo) * seg / kWarps);
-            const int end = (int)(lo + (hi - lo) * (seg + 1) / kWarps);
+            const double segs = lane < kWarps ? s_warp[lane] : 0.0;
+            const uint32_t over_at = __ballot_sync(0xffffffffu, segs > 0.0 && before + run_to > threshold);
+            const uint32_t some_at = __ballot_sync(0xffffffffu, segs > 0.0);
+            const int seg = over_at != 0 ? __ffs(over_at) - 1 : 31 - __clz(some_at);
+            double run = before + (seg > 0 ? __shfl_sync(0xffffffffu, run_to, seg - 1) : 0.0);
+            const int first = segment(seg), end = segment(seg + 1);
+            const int hits = DRAFT ? 0 : collect(first, end, gone);
             int found = -1, latest = -1;  // latest: last element with anything in it
             for (int v0 = first; v0 < end && found < 0; v0 += 32) {
                 double r[VE];
                 double sum = 0.0;
 #pragma unroll
                 for (int i = 0; i < VE; ++i) r[i] = 0.0;
-                if (v0 + lane < end) residual(v0 + lane, cc, gone, r);
+                if (v0 + lane < end) residual(v0 + lane, cc, hits, r);
                 int here = -1;
 #pragma unroll
                 for (int i = 0; i < VE; ++i) {
@@ -385,6 +480,14 @@ __global__ void __launch_bounds__(kThreads) tree_verify_kernel(const VerifyArgs 
             }
         }
         break;
+    }
+    if ((!agreed || n == 0) && rank == 0) {
+        if (!agreed && tid == 0) raise_bad_input(a.status);
+        if (tid < a.tokens) a.path[(int64_t)b * a.tokens + tid] = -1;
+        if (tid == 0) {
+            a.kept[b] = 0;
+            a.next_token[b] = -1;
+        }
     }
     // No CTA may leave while another still reads its sums.
     cluster_sync_all();
@@ -448,7 +551,16 @@ extern "C" int gqa_tree_verify(const gqa_tree_verify_params* p) {
     a.target_seq = p->target_seq_stride != 0 ? p->target_seq_stride : a.target_node * p->tokens;
     a.draft_seq = p->draft_seq_stride != 0 ? p->draft_seq_stride : a.draft_node * p->tokens;
     if (a.target_node < 0 || a.draft_node < 0 || a.target_seq < 0 || a.draft_seq < 0) return GQA_ERR_SHAPE;
-    a.cluster = kMaxCluster;
+    // As many CTAs per sequence as leave every lane two vectors of a row and run all at once (two per
+    // SM), at most 8 (portable clusters).
+    int32_t sms = 0;
+    if (current_sm_count(&sms) != GQA_OK) return GQA_ERR_CUDA;
+    const int64_t vectors = (int64_t)p->vocab * (int64_t)eb / 16;
+    a.cluster = 1;
+    while (a.cluster < kMaxCluster && vectors > (int64_t)2 * a.cluster * kThreads &&
+           (int64_t)2 * a.cluster * a.batch <= 2 * sms) {
+        a.cluster *= 2;
+    }
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(p->stream);
     cudaError_t e;
     if (p->dtype == GQA_DTYPE_F32) {

@@ -42,6 +42,26 @@ def test_struct_layouts_match_the_header(gqa, tmp_path):
             assert int(got[f"{name}.{field}"]) == getattr(mirror, field).offset, (name, field)
 
 
+def test_packed_blocks_match_the_structs(gqa):
+    """The blocks the binding packs in one go have every field where the structures have it."""
+    from llminfer_b200 import binding as B
+
+    def flat(kind):
+        for name, t in kind._fields_:
+            yield from (((name, f) for f, _ in t._fields_) if t is B._Layout else ((name,),))
+
+    for block, kind in ((B._ROPE, B._RopeParams), (B._TREE_DECODE, B._TreeDecodeParams),
+                        (B._TREE_VERIFY, B._TreeVerifyParams), (B._TREE_COMMIT, B._TreeCommitParams)):
+        names = list(flat(kind))
+        assert block.size == C.sizeof(kind)
+        p = kind.from_buffer_copy(block.pack(*range(1, len(names) + 1)))
+        for i, name in enumerate(names):
+            v = p
+            for f in name:
+                v = getattr(v, f)
+            assert v == i + 1, name
+
+
 @pytest.mark.parametrize("tokens", [1, 2, 31, 32, 33, 64, 127, 128])
 def test_masks_and_depths(gqa, tokens):
     rng = np.random.default_rng(tokens)
