@@ -13,8 +13,7 @@
 // share every key tile. While one stream computes weights, the tensor cores work for the other:
 //   S(j) .. weights(j) .. O += P(j) V, then S(j + 2) of the same stream, whose S and P share columns.
 // Warps 0-7: softmax, warp 8: bulk copies of Q, K and V into 128-byte swizzled rows (a ring of 32 KiB
-// tiles), warp 9: its lane 0 issues the products (warps 10 and 11 only complete the warpgroup whose registers
-// the softmax warps take over).
+// tiles), warp 9: its lane 0 issues the products.
 //
 // Work. All units (sequence, KV head, run of tokens) put their key tiles in one flat sequence that is cut evenly
 // over one CTA per SM, whatever the lengths are: few rows over a long history fill the GPU as well as
@@ -42,8 +41,7 @@ constexpr int kTileBytes = kTile * kHeadDim * 2;
 constexpr int kHalfBytes = kTileBytes / 2;      // 64 channels
 constexpr int kSlots = 6;                       // query tiles and ring together
 constexpr int kSoftmaxThreads = 256;
-constexpr int kThreads = kSoftmaxThreads + 128;
-constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;  // 256 * 224 + 128 * 56 = 384 * 168, what a launch gets
+constexpr int kThreads = kSoftmaxThreads + 64;
 constexpr int kUnitPad = 1;                     // places a unit counts on top of its tiles
 constexpr float kLazyMax = 8.0f;                // log2 of how far a score may exceed m
 constexpr uint64_t kWaitNs = 2000000000ull;
@@ -91,6 +89,15 @@ __device__ __forceinline__ bool meet(bool ok) {
     return all != 0;
 }
 
+// x / d for 0 <= x < 2^30, d > 0 and quotients below 2^21: every role divides a few times before its first
+// instruction of use, alone in its warp, where the general division is a chain of a hundred cycles.
+__device__ __forceinline__ int fast_div(int x, int d) {
+    int q = __float2int_rz(__fdividef((float)x, (float)d));  // off by at most one
+    const int r = x - q * d;
+    q += r >= d ? 1 : 0;
+    return r < 0 ? q - 1 : q;
+}
+
 // ---- the flat sequence of key tiles -------------------------------------------------------------
 struct Tables {
     int32_t* len;   // [batch] keys (0: nothing to do)
@@ -102,9 +109,15 @@ __device__ __forceinline__ Tables tables_at(int32_t* smem, int batch) {
 }
 size_t table_bytes(int batch) { return (3 * (size_t)batch + 1) * sizeof(int32_t); }
 
-template <int QT>  // query tiles per unit
+// Runs of tokens (units per KV head) of a tree of n > 0 nodes; QT: query tiles per unit.
+template <int QT>
+__device__ __forceinline__ int runs_of(const TreeArgs& a, int n) {
+    const int run = a.tile_tokens * QT;
+    return n <= run ? 1 : fast_div(n + run - 1, run);
+}
+template <int QT>
 __device__ __forceinline__ int units_of(const TreeArgs& a, int n) {
-    return a.num_kv_heads * ceil_div(n, a.tile_tokens * QT);
+    return a.num_kv_heads * runs_of<QT>(a, n);
 }
 __device__ __forceinline__ int places_of(int len) { return ceil_div(len, kTile) + kUnitPad; }
 
@@ -139,8 +152,8 @@ __device__ void build_tables(const TreeArgs& a, const Tables& t) {
     __syncthreads();
 }
 
-// The places cut over the CTAs: the first `extra` take per + 1 places, the others per; none without a
-// place takes part. 32-bit arithmetic: every role does this before its first instruction of use.
+// The places cut over the CTAs: the first `extra` take per + 1 places, the others per; no more CTAs take
+// part than get two places each (one tile for each stream: fewer records to merge). 32-bit arithmetic: every role does this before its first instruction of use.
 struct Cut {
     int total;
     int ctas;
@@ -149,13 +162,13 @@ struct Cut {
     __device__ int begin(int c) const { return c >= ctas ? total : c * per + min(c, extra); }
     __device__ int owner(int place) const {
         const int wide = extra * (per + 1);
-        return place < wide ? place / (per + 1) : extra + (place - wide) / per;
+        return place < wide ? fast_div(place, per + 1) : extra + fast_div(place - wide, per);
     }
 };
 __device__ __forceinline__ Cut cut_of(const TreeArgs& a, const Tables& t) {
     Cut c;
     c.total = t.base[a.batch];
-    c.ctas = min(a.ctas, c.total);
+    c.ctas = min(a.ctas, (c.total + 1) / 2);
     c.per = c.ctas > 0 ? c.total / c.ctas : 0;
     c.extra = c.total - c.per * c.ctas;
     return c;
@@ -183,9 +196,9 @@ __device__ __forceinline__ Unit unit_at(const TreeArgs& a, const Tables& t, int 
     u.len = t.len[lo];
     u.n = t.n[lo];
     const int per = places_of(u.len);
-    const int i = (place - t.base[lo]) / per;
-    const int runs = ceil_div(u.n, a.tile_tokens * QT);
-    u.hk = i / runs;
+    const int i = fast_div(place - t.base[lo], per);
+    const int runs = runs_of<QT>(a, u.n);
+    u.hk = runs == 1 ? i : fast_div(i, runs);
     u.token0 = (i - u.hk * runs) * a.tile_tokens * QT;
     u.tokens = min(u.n - u.token0, a.tile_tokens * QT);
     u.place = t.base[lo] + i * per;
@@ -276,6 +289,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&map_v);
     }
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), kColumns);
+    const int row_token = (threadIdx.x & 127) / a.group;  // of a softmax thread's row, inside its tile
+    const int row_head = (threadIdx.x & 127) - row_token * a.group;
     pdl_wait();
     pdl_launch_dependents();
     build_tables<QT>(a, tables);
@@ -290,9 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One query tile: the streams take key tiles in turn; two: both take every key tile.
     auto two_tiles = [&](const Unit& u) { return QT == 2 && u.tokens > a.tile_tokens; };
 
-    if (warp >= 8) {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-      if (warp == 8) {
+    if (warp == 8) {
         // ---- bulk copies ---------------------------------------------------------------------------
         const uint64_t policy = l2_policy_evict_first();
         const int boxes = kTile / a.box_keys;
@@ -340,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tok = key;
                         blk = a.cache.fixed_block;
                         if (a.cache.block_table != nullptr) {
-                            const int lb = key / a.cache.block_tokens;
+                            const int lb = fast_div(key, a.cache.block_tokens);
                             tok = key - lb * a.cache.block_tokens;
                             blk = __ldg(a.cache.block_table + (int64_t)p.u.b * a.cache.blocks_per_seq + lb);
                             if ((uint32_t)blk >= (uint32_t)a.cache.num_blocks) {
@@ -381,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         }
-      } else if (warp == 9) {
+    } else if (warp == 9) {
         // ---- products ------------------------------------------------------------------------------
         if (lane == 0) {
             constexpr uint32_t kShapeS = mma_shape(kTile, kTile, false);
@@ -421,12 +434,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < count && ok; ++j) {
                     const int st = j & 1, t = two ? j >> 1 : j;
                     const uint32_t f = ring_pos + order.v(t), slot = f % kRing;
-                    ok = wait_bar(smem_u32(&s_p_ready[st]), jobs[st] & 1u, dead) &&
-                         wait_bar(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
-                    ++jobs[st];
+                    ok = wait_bar(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
                     if (ok && j < 2 && pieces[st] > 0) {  // the last piece's O has been read
                         ok = wait_bar(smem_u32(&s_o_free[st]), (pieces[st] - 1) & 1u, dead);
                     }
+                    ok = ok && wait_bar(smem_u32(&s_p_ready[st]), jobs[st] & 1u, dead);
+                    ++jobs[st];
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t v = matrix_lo(ring + slot * kTileBytes, kHalfBytes);
@@ -454,9 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-      }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // ---- weights ---------------------------------------------------------------------------------
         const int st = warp >> 2;             // stream
         const int row = threadIdx.x & 127;    // of the stream's query tile; lane of tensor memory
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool two = two_tiles(p.u);
             const int count = two ? 2 * p.tiles : p.tiles;
             const Order order = {p.tiles, two ? 1 : 2};
-            const int in_unit = row / a.group + (two ? st * a.tile_tokens : 0);
+            const int in_unit = row_token + (two ? st * a.tile_tokens : 0);
             const int token = p.u.token0 + in_unit;
             const bool live = row < a.tile_tokens * a.group && in_unit < p.u.tokens;
             const bool any_live = __any_sync(0xffffffffu, live);
@@ -510,31 +521,64 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 tc_fence_after();
                 const bool tail = key0 + kTile > base;
-                if (any_live) {
-                    uint32_t s[4][32];
+                if (tail) {
+                    // V: rows past the end become zeros, rows of nodes are looked over.
+                    const uint32_t f = ring_pos + order.v(t), slot = f % kRing;
+                    ok = wait_warp(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
+                    if (!ok) break;
+                    const int key = key0 + row;
+                    uint4* v = reinterpret_cast<uint4*>(ring_ptr + slot * kTileBytes + row * 128);
+                    bool clear = key >= p.u.len;
+                    if (key >= base && !clear) {
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i) {
+                            const uint4 x = v[(i >> 3) * (kHalfBytes / 16) + (i & 7)];
+                            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_load32(my_s + 32 * c, s[c]);
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_loaded(s[c]);
-                    if (tail) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const uint32_t sees = live ? window(key0 + 32 * c - base) : 0u;
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                if (!(sees >> i & 1u)) s[c][i] = 0xff800000u;
+                            for (int c = 0; c < 4; ++c) {
+                                clear = clear || (e[c] & 0x7f80u) == 0x7f80u || (e[c] & 0x7f800000u) == 0x7f800000u;
                             }
                         }
-                        __syncwarp();
+                        if (clear) atomicOr(&s_bad[turn & 1][(key - base) >> 5], 1u << ((key - base) & 31));
                     }
-                    float top[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        top[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-                        for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+                    if (clear) {
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i) v[(i >> 3) * (kHalfBytes / 16) + (i & 7)] = make_uint4(0, 0, 0, 0);
                     }
-                    const float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    fence_proxy_async();
+                }
+                if (any_live) {
+                    // Rolled loops over 64 columns, read from tensor memory twice: the whole body stays in the
+                    // instruction cache next to the warp (128 columns in registers and unrolled ran at half the rate).
+                    if (tail) {
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t sees = live ? window(key0 + 32 * c - base) : 0u;
+                            uint32_t s[32];
+                            __syncwarp();
+                            tmem_load32(my_s + 32 * c, s);
+                            tmem_loaded(s);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                if (!(sees >> i & 1u)) s[i] = 0xff800000u;
+                            }
+                            tmem_store32(my_s + 32 * c, s);
+                        }
+                        tmem_stored();
+                    }
+                    float mx = -INFINITY;
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t s[2][32];
+                        tmem_load32(my_s + 64 * half, s[0]);
+                        tmem_load32(my_s + 64 * half + 32, s[1]);
+                        tmem_loaded(s[0]);
+                        tmem_loaded(s[1]);
+                        float top[4] = {mx, mx, mx, mx};
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i >> 5][i & 31]));
+                        mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    }
                     if (j < 2) {
                         m = mx;
                     } else {
@@ -561,49 +605,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     const float off = safe_max(m) * scale;
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
+#pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
-                        uint32_t w[32];
+                        uint32_t s[2][32], w[32];
+                        tmem_load32(my_s + 64 * half, s[0]);
+                        tmem_load32(my_s + 64 * half + 32, s[1]);
+                        tmem_loaded(s[0]);
+                        tmem_loaded(s[1]);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const float e0 = ex2_approx(__uint_as_float(s[2 * half + c][2 * i]) * scale - off);
-                                const float e1 = ex2_approx(__uint_as_float(s[2 * half + c][2 * i + 1]) * scale - off);
-                                sum[i & 3] += e0 + e1;
-                                w[16 * c + i] = pack_bf16(e0, e1);
-                            }
+                        for (int i = 0; i < 32; ++i) {
+                            const float e0 = ex2_approx(__uint_as_float(s[i >> 4][2 * i & 31]) * scale - off);
+                            const float e1 = ex2_approx(__uint_as_float(s[i >> 4][(2 * i & 31) + 1]) * scale - off);
+                            sum[i & 3] += e0 + e1;
+                            w[i] = pack_bf16(e0, e1);
                         }
                         tmem_store32(my_s + 32 * half, w);
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tmem_stored();
-                }
-                if (tail) {
-                    // V: rows past the end become zeros, rows of nodes are looked over.
-                    const uint32_t f = ring_pos + order.v(t), slot = f % kRing;
-                    ok = wait_warp(smem_u32(&s_kv_full[slot]), (f / kRing) & 1u, dead);
-                    if (!ok) break;
-                    const int key = key0 + row;
-                    uint4* v = reinterpret_cast<uint4*>(ring_ptr + slot * kTileBytes + row * 128);
-                    bool clear = key >= p.u.len;
-                    if (key >= base && !clear) {
-#pragma unroll 1
-                        for (int i = 0; i < 16; ++i) {
-                            const uint4 x = v[(i >> 3) * (kHalfBytes / 16) + (i & 7)];
-                            const uint32_t e[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                clear = clear || (e[c] & 0x7f80u) == 0x7f80u || (e[c] & 0x7f800000u) == 0x7f800000u;
-                            }
-                        }
-                        if (clear) atomicOr(&s_bad[turn & 1][(key - base) >> 5], 1u << ((key - base) & 31));
-                    }
-                    if (clear) {
-#pragma unroll 1
-                        for (int i = 0; i < 16; ++i) v[(i >> 3) * (kHalfBytes / 16) + (i & 7)] = make_uint4(0, 0, 0, 0);
-                    }
-                    fence_proxy_async();
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -638,7 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (any_live) {
                 const int chunk0 = two ? 0 : 2 * st, chunks = two ? 4 : 2;
                 const float inv = l_row == 0.0f ? 0.0f : 1.0f / l_row;
-                const int head = p.u.hk * a.group + row % a.group;
+                const int head = p.u.hk * a.group + row_head;
                 __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
                                      (mask_row * a.num_q_heads + head) * kHeadDim;
                 float* rec = a.workspace + ((int64_t)(2 * blockIdx.x + (p.tile == 0 ? 1 : 0)) * QT + (two ? st : 0)) *
@@ -730,21 +749,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 // 4 (tid / 8) .. + 3.
 template <int QT>
 __global__ void __launch_bounds__(256, 4) tree_merge_kernel(const TreeArgs a) {
-    pdl_launch_dependents();
-    pdl_wait();
-    const int4 head = __ldcg(a.cut_units + 2 * blockIdx.x);
-    const int c0 = blockIdx.x, c1 = head.x;
-    if (c1 < 0) return;
-    struct {
-        int b, hk, token0, tokens;
-    } u = {head.y, head.z, head.w, __ldcg(a.cut_units + 2 * blockIdx.x + 1).x};
-    const int tiles_rows = a.tile_tokens * a.group;
     const int r = blockIdx.y * 8 + (threadIdx.x & 7);  // row of the unit
-    if (r >= u.tokens * a.group) return;
-    const int tile = r / tiles_rows, row = r - tile * tiles_rows;
+    const int tile_rows = a.tile_tokens * a.group;
+    const int tile = r >= tile_rows ? 1 : 0, row = r - tile * tile_rows;
     const int chunk = threadIdx.x >> 3;
+    const int token = r / a.group;  // of the unit
     const int64_t record = (int64_t)QT * a.tile_rows * kRecordCols;
     const float* rec = a.workspace + (int64_t)tile * a.tile_rows * kRecordCols;
+    const int c0 = blockIdx.x;
+    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (r - token * a.group) * kHeadDim + chunk * 4;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int4 head = __ldcg(a.cut_units + 2 * c0);  // last CTA, sequence, KV head, first token
+    const int c1 = head.x;
+    if (c1 < 0 || token >= __ldcg(a.cut_units + 2 * c0 + 1).x) return;
     auto at = [&](int c) { return rec + (int64_t)(2 * c + (c == c0 ? 1 : 0)) * record; };
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -778,10 +796,7 @@ __global__ void __launch_bounds__(256, 4) tree_merge_kernel(const TreeArgs a) {
         m = next;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int token = u.token0 + r / a.group;
-    __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) +
-                         (((int64_t)u.b * a.cache.tokens + token) * a.num_q_heads + u.hk * a.group + r % a.group) *
-                             kHeadDim + chunk * 4;
+    out += (((int64_t)head.y * a.cache.tokens + head.w + token) * a.num_q_heads + head.z * a.group) * kHeadDim;
     *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
 }
 

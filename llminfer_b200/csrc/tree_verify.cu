@@ -16,8 +16,8 @@
 // a CTA contiguous segments of its slice. Every CTA walks the tree itself (same inputs, same sums,
 // same steps); after a pass the CTAs read one another's partial sums through distributed shared
 // memory. To place the sample, the partial sums name the segment in which the cumulative sum
-// passes u S, and one warp walks that segment again. A pass is bound by the latency of its loads: a lane
-// has four vectors in flight.
+// passes u S, the kept sums of its rounds the round of 32 vectors, and one warp looks through that. A pass is bound by the latency of its loads: a lane
+// has eight vectors of each row in flight (two: 4.4 us a pass over 16000 elements per CTA).
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -31,6 +31,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
+constexpr int kMaxRounds = 64;  // rounds of 32 vectors of a warp's segment whose sums are kept
 constexpr int kWords = kTreeMaxTokens / 32;
 
 struct VerifyArgs {
@@ -49,7 +50,8 @@ struct VerifyArgs {
     int32_t batch;
     int32_t tokens;
     int32_t vocab;
-    int32_t cluster;
+    int32_t cluster;  // a power of two
+    int32_t cluster_log2;
 };
 
 __device__ __forceinline__ float value(const float* p) { return __ldg(p); }
@@ -70,17 +72,44 @@ __device__ __forceinline__ void elements(uint4 u, float (&x)[8]) {
     }
 }
 
-// An FP32 number as FP64, by its bits: the conversion instruction runs at a quarter of the rate of FP64
-// arithmetic and would bound a pass. Negative numbers, NaN and numbers below 2^-126 give 0, infinity 2^128.
-__device__ __forceinline__ double widen(float x) {
-    const uint32_t u = __float_as_uint(fmaxf(x, 0.0f));
-    const bool some = u >= 0x00800000u;
-    return __hiloint2double(some ? (int)((u >> 3) + 0x38000000u) : 0, some ? (int)(u << 29) : 0);
-}
-// max(p - c q, 0)
+// max(p - c q, 0); NaN and negative entries count as 0. The two conversions (8 cycles per warp each, as
+// measured, where the bit operations that could replace one take 14) bound a pass.
 __device__ __forceinline__ double rest_of(float p, float q, double c) {
-    const double r = fma(-c, widen(q), widen(p));
-    return __double2hiint(r) < 0 ? 0.0 : r;
+    const double r = fma(-c, (double)fmaxf(q, 0.0f), (double)p);
+    return r > 0.0 ? r : 0.0;
+}
+__device__ __forceinline__ double rest_of(float p) { return (double)fmaxf(p, 0.0f); }
+
+// The sums over the warp of eight values per lane: lane 4 k of a warp gets that of value k. Halves of the values
+// change places with each step: 9 exchanges instead of 40.
+__device__ __forceinline__ double reduce8(const double (&v)[8], int lane) {
+    double a[4], b[2], c;
+    const bool h16 = lane & 16, h8 = lane & 8, h4 = lane & 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        a[i] = (h16 ? v[i + 4] : v[i]) + __shfl_xor_sync(0xffffffffu, h16 ? v[i] : v[i + 4], 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        b[i] = (h8 ? a[i + 2] : a[i]) + __shfl_xor_sync(0xffffffffu, h8 ? a[i] : a[i + 2], 8);
+    }
+    c = (h4 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, h4 ? b[0] : b[1], 4);
+    c += __shfl_xor_sync(0xffffffffu, c, 2);
+    return c + __shfl_xor_sync(0xffffffffu, c, 1);
+}
+
+// In pairs: an FP64 sum is a chain of long latencies otherwise.
+template <int N>
+__device__ __forceinline__ double sum_of(const double (&r)[N]) {
+    double s[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) s[i] = r[2 * i] + r[2 * i + 1];
+#pragma unroll
+    for (int n = N / 2; n > 1; n /= 2) {
+#pragma unroll
+        for (int i = 0; i < n / 2; ++i) s[i] = s[2 * i] + s[2 * i + 1];
+    }
+    return s[0];
 }
 
 // Where the walk stands.
@@ -114,19 +143,21 @@ __device__ __forceinline__ Said ld_cluster_said(uint32_t addr) {
 }
 
 template <typename T, bool DRAFT>
-__global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) tree_verify_kernel(const VerifyArgs a) {
     constexpr int VE = 16 / (int)sizeof(T);
-    constexpr int kUnroll = DRAFT ? 2 : 4;  // vectors of a row a lane has in flight
+    constexpr int kUnroll = 8;  // vectors of a row a lane has in flight
     __shared__ uint32_t s_child[kTreeMaxTokens][kWords];
     __shared__ float s_p[kTreeMaxTokens], s_q[kTreeMaxTokens], s_u[kTreeMaxTokens];
     __shared__ int32_t s_word[kTreeMaxTokens];
     __shared__ int32_t s_path[kTreeMaxTokens];
+    __shared__ uint8_t s_first[kTreeMaxTokens];        // passes the test that holds before a rejection
     __shared__ uint8_t s_again[kTreeMaxTokens];        // an earlier sibling has the same token
     __shared__ double s_ahead[kTreeMaxTokens];         // p at the tokens of later siblings
     __shared__ int32_t s_gone[kTreeMaxTokens];         // tokens left out of the sum (no draft)
     __shared__ uint8_t s_hit[kWarps][kTreeMaxTokens];  // those inside a warp's segment
     __shared__ int s_gone_count;
     __shared__ double s_warp[kWarps];
+    __shared__ double s_round[kWarps][kMaxRounds];  // sums of the rounds of the last pass
     __shared__ Said s_said[2];  // this CTA's sum and step, buffers in turn: read by the whole cluster
     __shared__ Walk w;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -166,6 +197,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
         s_u[tid] = u;
         s_p[tid] = p;
         s_q[tid] = q;
+        s_first[tid] = (double)u * (double)fmaxf(q, 0.0f) < rest_of(p);
     }
     bad = __syncthreads_or(bad);
     if (bad && rank == 0 && tid == 0) raise_bad_input(a.status);
@@ -189,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
     double total = 0.0;      // sum of the residual after the last pass
     double before = 0.0;     // of the CTAs before this one
     double own = 0.0;
-    bool later = false;      // a CTA after this one has something in its slice
+    double parts = 0.0, upto = 0.0;  // lane k: CTA k's sum, and the sum up to it
     double run_to = 0.0;     // lane i: sum of this CTA's segments 0 .. i
     // The row in vectors of 16 bytes. A vector is cut at the row's ends, where single elements are
     // read; rows p and q that are not equally aligned are read element by element.
@@ -203,10 +235,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
         wide = !DRAFT || ((reinterpret_cast<uintptr_t>(p_row) ^ reinterpret_cast<uintptr_t>(q_row)) & 15u) == 0;
         vecs = (a.vocab + shift + VE - 1) / VE;
     };
-    // First vector of segment `seg` of this CTA's slice.
+    // First vector of segment `seg` of this CTA's slice (slices and segments of equal length but the last:
+    // shifts, where an exact cut would take four 64-bit divisions, 0.9 us ahead of the first load).
     auto segment = [&](int seg) -> int {
-        const int64_t lo = (int64_t)vecs * rank / a.cluster, hi = (int64_t)vecs * (rank + 1) / a.cluster;
-        return (int)(lo + (hi - lo) * seg / kWarps);
+        const int slice = (vecs + a.cluster - 1) >> a.cluster_log2;
+        const int part = (slice + kWarps - 1) / kWarps;
+        const int lo = min(vecs, rank * slice), hi = min(vecs, lo + slice);
+        return min(hi, lo + seg * part);
     };
     // The tokens left out that lie in vectors [first, end), into this warp's list.
     auto collect = [&](int first, int end, int gone) -> int {
@@ -227,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
     auto rest = [&](int vec, const float (&p)[VE], const float (&q)[VE], double c, int hits, double (&r)[VE]) {
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-            r[i] = DRAFT && c > 0.0 ? rest_of(p[i], q[i], c) : widen(p[i]);
+            r[i] = DRAFT && c > 0.0 ? rest_of(p[i], q[i], c) : rest_of(p[i]);
         }
         if (!DRAFT) {
             for (int k = 0; k < hits; ++k) {
@@ -263,18 +298,20 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
                               (uint64_t)w.action << 24 | (uint64_t)(uint32_t)turn << 32;
         if (tid == 0) s_said[turn & 1] = Said{own, step};
         cluster_sync_all();
-        total = before = 0.0;
-        later = false;
-        bool agreed = true;
-        uint64_t lead = 0;
-        for (int k = 0; k < a.cluster; ++k) {
-            const Said said = ld_cluster_said(cluster_map(smem_u32(&s_said[turn & 1]), (uint32_t)k));
-            if (k == 0) lead = said.step;
-            agreed = agreed && said.step == lead;
-            if (k < rank) before += said.sum;
-            later = later || (k > rank && said.sum > 0.0);
-            total += said.sum;
+        // Lane k reads CTA k; running sums by a scan, the same operations on the same numbers in every CTA.
+        const bool one = lane < a.cluster;
+        Said said = {0.0, 0};
+        if (one) said = ld_cluster_said(cluster_map(smem_u32(&s_said[turn & 1]), (uint32_t)lane));
+        parts = said.sum;
+        upto = said.sum;
+#pragma unroll
+        for (int d = 1; d < kMaxCluster; d <<= 1) {
+            const double up = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += up;
         }
+        total = __shfl_sync(0xffffffffu, upto, a.cluster - 1);
+        before = rank > 0 ? __shfl_sync(0xffffffffu, upto, rank - 1) : 0.0;
+        const bool agreed = __all_sync(0xffffffffu, !one || said.step == step);
         ++turn;
         return agreed;
     };
@@ -282,20 +319,21 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
         const int lo = segment(warp), hi = segment(warp + 1);
         const int hits = DRAFT ? 0 : collect(lo, hi, gone);
         double sum = 0.0;
-        for (int v0 = lo + lane; v0 < hi; v0 += 32 * kUnroll) {
-            // The ends of the row are cut off here and added below.
+        for (int v0 = lo; v0 < hi; v0 += 32 * kUnroll) {
             uint4 up[kUnroll], uq[kUnroll];
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
-                const int vec = v0 + 32 * k;
+                const int vec = v0 + 32 * k + lane;
                 if (vec < hi && wide && whole(vec)) {
                     up[k] = __ldg(reinterpret_cast<const uint4*>(p_row + (vec * VE - shift)));
                     if (DRAFT && c > 0.0) uq[k] = __ldg(reinterpret_cast<const uint4*>(q_row + (vec * VE - shift)));
                 }
             }
+            double round[kUnroll];
 #pragma unroll
             for (int k = 0; k < kUnroll; ++k) {
-                const int vec = v0 + 32 * k;
+                round[k] = 0.0;
+                const int vec = v0 + 32 * k + lane;
                 if (vec >= hi) continue;
                 double r[VE];
                 if (wide && whole(vec)) {
@@ -306,9 +344,13 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
                 } else {
                     residual(vec, c, hits, r);
                 }
-#pragma unroll
-                for (int i = 0; i < VE; ++i) sum += r[i];
+                round[k] = sum_of(r);
             }
+            __syncwarp();
+            const double of = reduce8(round, lane);  // lane 4 k: round k
+            const int at = (v0 - lo) / 32 + (lane >> 2);
+            if ((lane & 3) == 0 && at < kMaxRounds) s_round[warp][at] = of;
+            sum += sum_of(round);
         }
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -325,6 +367,46 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
         const bool agreed = exchange();
         __syncthreads();
         return agreed;
+    };
+    // One warp: the element of vectors [first, end) at which the running sum (`run` before them) passes the
+    // threshold, else the last one with anything in it, else -1.
+    auto place = [&](int first, int end, double run, double threshold, double c, int hits) -> int {
+        int found = -1, latest = -1;  // latest: last element with anything in it
+        for (int v0 = first; v0 < end && found < 0; v0 += 32) {
+            double r[VE];
+            double sum = 0.0;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) r[i] = 0.0;
+            if (v0 + lane < end) residual(v0 + lane, c, hits, r);
+            int here = -1;
+#pragma unroll
+            for (int i = 0; i < VE; ++i) {
+                sum += r[i];
+                if (r[i] > 0.0) here = (v0 + lane) * VE - shift + i;
+            }
+            double incl = sum;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const double up = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += up;
+            }
+            const uint32_t over = __ballot_sync(0xffffffffu, run + incl > threshold && sum > 0.0);
+            const uint32_t some = __ballot_sync(0xffffffffu, here >= 0);
+            if (over != 0) {
+                double at = run + (incl - sum);
+                int pick = -1;
+#pragma unroll
+                for (int i = 0; i < VE; ++i) {
+                    at += r[i];
+                    if (pick < 0 && r[i] > 0.0 && at > threshold) pick = (v0 + lane) * VE - shift + i;
+                }
+                found = __shfl_sync(0xffffffffu, pick >= 0 ? pick : here, __ffs(over) - 1);
+            } else if (some != 0) {
+                latest = __shfl_sync(0xffffffffu, here, 31 - __clz(some));
+            }
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        return found >= 0 ? found : latest;
     };
     // The child of w.node after w.tried, -1: none.
     auto next_child = [&]() -> int {
@@ -349,9 +431,15 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
                     break;
                 }
                 w.tried = child;
-                const double room = DRAFT ? rest_of(s_p[child], w.c > 0.0 ? s_q[child] : 0.0f, w.c)
-                                          : s_again[child] ? 0.0 : widen(s_p[child]);
-                if ((double)s_u[child] * widen(s_q[child]) * w.sum < room) {
+                bool taken;
+                if (w.rejected == 0) {
+                    taken = s_first[child];
+                } else {
+                    const double room = DRAFT ? rest_of(s_p[child], s_q[child], w.c)
+                                              : s_again[child] ? 0.0 : rest_of(s_p[child]);
+                    taken = (double)s_u[child] * (double)fmaxf(s_q[child], 0.0f) * w.sum < room;
+                }
+                if (taken) {
                     w.node = child;
                     w.c = 0.0;
                     w.sum = 1.0;
@@ -380,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
                         s_ahead[at] = ahead;
                         if (!s_again[at]) {
                             s_gone[count++] = s_word[at];
-                            ahead += widen(s_p[at]);
+                            ahead += rest_of(s_p[at]);
                         }
                     }
                 }
@@ -416,9 +504,9 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
         // The first CTA whose running sum passes the threshold (or the last one with anything in it)
         // holds the sample; in it, likewise, the warp, the round of 32 vectors, the lane.
         const double threshold = (double)u_sample * total;
-        // The running sums are the same numbers in every CTA, so exactly one of them passes it.
-        const bool mine = total > threshold ? !(before > threshold) && before + own > threshold
-                                            : own > 0.0 && !later;
+        const uint32_t passed = __ballot_sync(0xffffffffu, lane < a.cluster && parts > 0.0 && upto > threshold);
+        const uint32_t filled = __ballot_sync(0xffffffffu, lane < a.cluster && parts > 0.0);
+        const bool mine = filled != 0 && (passed != 0 ? __ffs(passed) - 1 : 31 - __clz(filled)) == rank;
         if (mine && warp == 0) {
             const double segs = lane < kWarps ? s_warp[lane] : 0.0;
             const uint32_t over_at = __ballot_sync(0xffffffffu, segs > 0.0 && before + run_to > threshold);
@@ -427,45 +515,45 @@ __global__ void __launch_bounds__(kThreads, 2) tree_verify_kernel(const VerifyAr
             double run = before + (seg > 0 ? __shfl_sync(0xffffffffu, run_to, seg - 1) : 0.0);
             const int first = segment(seg), end = segment(seg + 1);
             const int hits = DRAFT ? 0 : collect(first, end, gone);
-            int found = -1, latest = -1;  // latest: last element with anything in it
-            for (int v0 = first; v0 < end && found < 0; v0 += 32) {
-                double r[VE];
-                double sum = 0.0;
+            int token = -1;
+            // First which round of the pass, then which element. Rounds beyond those kept are looked over.
+            const int rounds = (end - first + 31) / 32;
+            if (rounds > 1) {
+                double at = run;
+                int pick = -1, last = -1;
+                double pick_run = run, last_run = run;
+                for (int r0 = 0; r0 < min(rounds, kMaxRounds) && pick < 0; r0 += 32) {
+                    const int i = r0 + lane;
+                    const double sum = i < min(rounds, kMaxRounds) ? s_round[seg][i] : 0.0;
+                    double incl = sum;
 #pragma unroll
-                for (int i = 0; i < VE; ++i) r[i] = 0.0;
-                if (v0 + lane < end) residual(v0 + lane, cc, hits, r);
-                int here = -1;
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    sum += r[i];
-                    if (r[i] > 0.0) here = (v0 + lane) * VE - shift + i;
-                }
-                double incl = sum;
-#pragma unroll
-                for (int d = 1; d < 32; d <<= 1) {
-                    const double up = __shfl_up_sync(0xffffffffu, incl, d);
-                    if (lane >= d) incl += up;
-                }
-                const uint32_t over = __ballot_sync(0xffffffffu, run + incl > threshold && sum > 0.0);
-                const uint32_t some = __ballot_sync(0xffffffffu, here >= 0);
-                if (over != 0) {
-                    const int who = __ffs(over) - 1;
-                    double at = run + (incl - sum);
-                    int pick = here;
-#pragma unroll
-                    for (int i = VE - 1; i >= 0; --i) {
-                        double upto = at;
-#pragma unroll
-                        for (int j = 0; j <= i; ++j) upto += r[j];
-                        if (r[i] > 0.0 && upto > threshold) pick = (v0 + lane) * VE - shift + i;
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const double up = __shfl_up_sync(0xffffffffu, incl, d);
+                        if (lane >= d) incl += up;
                     }
-                    found = __shfl_sync(0xffffffffu, pick, who);
-                } else if (some != 0) {
-                    latest = __shfl_sync(0xffffffffu, here, 31 - __clz(some));
+                    const double ahead = at + (incl - sum);
+                    const uint32_t over = __ballot_sync(0xffffffffu, sum > 0.0 && at + incl > threshold);
+                    const uint32_t some = __ballot_sync(0xffffffffu, sum > 0.0);
+                    if (over != 0) {
+                        pick = r0 + __ffs(over) - 1;
+                        pick_run = __shfl_sync(0xffffffffu, ahead, __ffs(over) - 1);
+                    } else if (some != 0) {
+                        last = r0 + 31 - __clz(some);
+                        last_run = __shfl_sync(0xffffffffu, ahead, 31 - __clz(some));
+                    }
+                    at += __shfl_sync(0xffffffffu, incl, 31);
                 }
-                run += __shfl_sync(0xffffffffu, incl, 31);
+                if (pick < 0 && rounds > kMaxRounds) {
+                    token = place(first + 32 * kMaxRounds, end, at, threshold, cc, hits);
+                }
+                if (token < 0) {
+                    const int at_round = first + 32 * (pick >= 0 ? pick : max(last, 0));
+                    token = place(at_round, min(end, at_round + 32), pick >= 0 ? pick_run : last_run, threshold, cc, hits);
+                }
+            } else {
+                token = place(first, end, run, threshold, cc, hits);
             }
-            if (lane == 0) a.next_token[b] = found >= 0 ? found : latest;
+            if (lane == 0) a.next_token[b] = token;
         }
         if (rank == 0) {
             if (tid < a.tokens) {
@@ -551,15 +639,17 @@ extern "C" int gqa_tree_verify(const gqa_tree_verify_params* p) {
     a.target_seq = p->target_seq_stride != 0 ? p->target_seq_stride : a.target_node * p->tokens;
     a.draft_seq = p->draft_seq_stride != 0 ? p->draft_seq_stride : a.draft_node * p->tokens;
     if (a.target_node < 0 || a.draft_node < 0 || a.target_seq < 0 || a.draft_seq < 0) return GQA_ERR_SHAPE;
-    // As many CTAs per sequence as leave every lane two vectors of a row and run all at once (two per
+    // As many CTAs per sequence as leave every lane two vectors of a row and run all at once (one per
     // SM), at most 8 (portable clusters).
     int32_t sms = 0;
     if (current_sm_count(&sms) != GQA_OK) return GQA_ERR_CUDA;
     const int64_t vectors = (int64_t)p->vocab * (int64_t)eb / 16;
     a.cluster = 1;
+    a.cluster_log2 = 0;
     while (a.cluster < kMaxCluster && vectors > (int64_t)2 * a.cluster * kThreads &&
-           (int64_t)2 * a.cluster * a.batch <= 2 * sms) {
+           (int64_t)2 * a.cluster * a.batch <= sms) {
         a.cluster *= 2;
+        ++a.cluster_log2;
     }
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(p->stream);
     cudaError_t e;
