@@ -11,10 +11,8 @@
 // A block takes a token and some or all of its heads. Its threads compute the token's angles once, one pair each,
 // into shared memory; a warp then walks over its heads two at a time, 16 lanes per head. A lane holds two
 // groups of four channels: in the half pairing i .. i + 3 and their partners i + rotary_dim / 2 .., so that a rotation
-// stays inside the lane, else eight neighbours. (With one head per warp, partners fetched by
-// shuffles, the kernel was bound by instruction issue at 44 us for 3072 tokens of 80 heads, 0.43 of the measured copy
-// bandwidth.) The rows' addresses need neither lengths nor angles, so a warp asks for its kBatch
-// pairs of heads before it looks at either.
+// stays inside the lane, else eight neighbours. The rows' addresses need neither lengths nor angles, so
+// a warp asks for all its heads before it looks at either.
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -25,8 +23,9 @@
 namespace gqa {
 namespace {
 
-constexpr int kBatch = 4;      // pairs of heads of a warp, all in flight
-constexpr int kMaxWarps = 16;  // of a block
+constexpr int kMaxWarps = 8;  // of a block
+// Pairs of heads of a warp, all in flight: 64 bytes a lane.
+template <typename T> constexpr int kPairs = 32 / (int)sizeof(T) / 2;
 
 struct RopeArgs {
     TreeCache cache;
@@ -43,9 +42,11 @@ struct RopeArgs {
     int64_t q_out_stride;
     int64_t k_stride;
     int64_t v_stride;
+    int32_t batch;
     int32_t num_q_heads;
     int32_t num_kv_heads;
     int32_t rotary_dim;
+    int32_t pairs_per_warp;  // pairs of heads, kPairs at most
     int32_t heads_per_block;
     float eps;
     float attn_factor;
@@ -72,10 +73,11 @@ __device__ __forceinline__ void pack(const float (&x)[4], float4* u) {
     *u = make_float4(x[0], x[1], x[2], x[3]);
 }
 
-// grid.x: parts of a token's heads (queries, keys, values in this order); grid.y * grid.z: tokens.
+// grid.x: parts of a token's heads (queries, keys, values in this order); grid.y: tokens; grid.z: sequences.
 template <typename T, bool HALF, bool NORM>
-__global__ void __launch_bounds__(kMaxWarps * 32, 2) rope_append_kernel(const RopeArgs a, int32_t nodes) {
+__global__ void __launch_bounds__(kMaxWarps * 32, 3) rope_append_kernel(const RopeArgs a) {
     using R = typename Raw<T>::type;
+    constexpr int kBatch = kPairs<T>;
     __shared__ float s_cos[kHeadDim / 2], s_sin[kHeadDim / 2];
     __shared__ float s_weight[NORM ? 2 * kHeadDim : 1];
     const int warp = threadIdx.x >> 5;
@@ -83,35 +85,32 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) rope_append_kernel(const Ro
     const int warps = blockDim.x >> 5;
     const int heads = a.num_q_heads + 2 * a.num_kv_heads;
     const int keys_at = a.num_q_heads, values_at = a.num_q_heads + a.num_kv_heads;
-    const int bt = blockIdx.z * gridDim.y + blockIdx.y;
+    const int b = blockIdx.z, t = blockIdx.y;
+    const int bt = b * a.cache.tokens + t;
     pdl_launch_dependents();
-    if (bt >= nodes) return;
     const int end = min(heads, (int)(blockIdx.x + 1) * a.heads_per_block);
-    const int mine = blockIdx.x * a.heads_per_block + 2 * warp + (lane >> 4);  // this half warp's first head
+    // This half warp's heads: mine, mine + 2, ... (pairs_per_warp of them, the warps side by side).
+    const int mine = blockIdx.x * a.heads_per_block + 2 * a.pairs_per_warp * warp + (lane >> 4);
     // The lane's channels: g0 .. g0 + 3 and g1 .. g1 + 3.
     const int l = lane & 15;
     const bool rotated = l < (a.rotary_dim >> 3);
     const int g0 = HALF && rotated ? 4 * l : 8 * l;
     const int g1 = HALF && rotated ? g0 + (a.rotary_dim >> 1) : g0 + 4;
+    // Head h of the token lies at the base of its kind + 128 h.
+    const T* q_in = static_cast<const T*>(a.q) + bt * a.q_stride;
+    const T* k_in = static_cast<const T*>(a.k_new) + bt * a.k_stride - keys_at * kHeadDim;
+    const T* v_in = static_cast<const T*>(a.v_new) + bt * a.v_stride - values_at * kHeadDim;
     pdl_wait();
 
     R x[kBatch][2];
-    auto load = [&](int h0) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int h = h0 + 2 * i * warps;
-            if (h >= end) continue;
-            const T* src = h < keys_at ? static_cast<const T*>(a.q) + bt * a.q_stride + h * kHeadDim
-                           : h < values_at
-                               ? static_cast<const T*>(a.k_new) + bt * a.k_stride + (h - keys_at) * kHeadDim
-                               : static_cast<const T*>(a.v_new) + bt * a.v_stride + (h - values_at) * kHeadDim;
-            x[i][0] = *reinterpret_cast<const R*>(src + g0);
-            x[i][1] = *reinterpret_cast<const R*>(src + g1);
-        }
-    };
-    load(mine);
-    const int b = bt / a.cache.tokens;
-    const int t = bt - b * a.cache.tokens;
+    for (int i = 0; i < kBatch; ++i) {
+        const int h = mine + 2 * i;
+        if (h >= end || i >= a.pairs_per_warp) continue;
+        const T* src = (h < keys_at ? q_in : h < values_at ? k_in : v_in) + h * kHeadDim;
+        x[i][0] = *reinterpret_cast<const R*>(src + g0);
+        x[i][1] = *reinterpret_cast<const R*>(src + g1);
+    }
     const int pairs = a.rotary_dim >> 1;
     double freq = 0.0;
     if ((int)threadIdx.x < pairs) freq = __ldg(a.freq + threadIdx.x);
@@ -126,9 +125,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) rope_append_kernel(const Ro
     const TreeSpan span = tree_span(a.cache, b);
     if (!span.ok && t == 0 && blockIdx.x == 0 && threadIdx.x == 0) raise_bad_input(a.cache.status);
     if (t >= span.n) return;
-    int64_t row = 0;
-    const bool placed = tree_row(a.cache, b, span.base + t, &row);
-    if (!placed && blockIdx.x == 0 && threadIdx.x == 0) raise_bad_input(a.cache.status);
     if ((int)threadIdx.x < pairs) {
         const double turns = (double)(span.base + ahead) * (freq * 0.15915494309189533577);
         float sn, cs;
@@ -136,84 +132,123 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) rope_append_kernel(const Ro
         s_cos[threadIdx.x] = cs * a.attn_factor;
         s_sin[threadIdx.x] = sn * a.attn_factor;
     }
-    __syncthreads();
-    // The four pairs of the lane (channels that are not rotated turn by nothing).
-    float cs[4], sn[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        cs[i] = rotated ? s_cos[4 * l + i] : 1.0f;
-        sn[i] = rotated ? s_sin[4 * l + i] : 0.0f;
-    }
-
-#pragma unroll 1
-    for (int h0 = mine; h0 - (lane >> 4) < end; h0 += 2 * kBatch * warps) {
-        if (h0 != mine) load(h0);
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            const int h = h0 + 2 * i * warps;
-            const bool is_q = h < keys_at;
-            float scale = 1.0f;
-            float v[2][4];
-            unpack(x[i][0], v[0]);
-            unpack(x[i][1], v[1]);
-            if (NORM) {
-                // Both halves of the warp take part, whatever their heads are.
-                float sum = 0.0f;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) sum += v[0][c] * v[0][c] + v[1][c] * v[1][c];
-#pragma unroll
-                for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                scale = rsqrtf(sum * (1.0f / kHeadDim) + a.eps);
-            }
-            if (h >= end) continue;
-            if (h < values_at) {
-                if (NORM) {
-                    const float* w = s_weight + (is_q ? 0 : kHeadDim);
-                    const float4 w0 = *reinterpret_cast<const float4*>(w + g0);
-                    const float4 w1 = *reinterpret_cast<const float4*>(w + g1);
-                    v[0][0] *= scale * w0.x; v[0][1] *= scale * w0.y; v[0][2] *= scale * w0.z; v[0][3] *= scale * w0.w;
-                    v[1][0] *= scale * w1.x; v[1][1] *= scale * w1.y; v[1][2] *= scale * w1.z; v[1][3] *= scale * w1.w;
-                }
-                float y[2][4];
-                if (HALF) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        y[0][c] = v[0][c] * cs[c] - v[1][c] * sn[c];
-                        y[1][c] = v[0][c] * sn[c] + v[1][c] * cs[c];
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int g = c >> 1, at = 2 * (c & 1);
-                        y[g][at] = v[g][at] * cs[c] - v[g][at + 1] * sn[c];
-                        y[g][at + 1] = v[g][at] * sn[c] + v[g][at + 1] * cs[c];
-                    }
-                }
-                pack(y[0], &x[i][0]);
-                pack(y[1], &x[i][1]);
-            }
-            T* dst;
-            if (is_q) {
-                dst = static_cast<T*>(a.q_out) + bt * a.q_out_stride + h * kHeadDim;
-            } else if (placed) {
-                dst = row + (h < values_at ? static_cast<T*>(a.k_cache) + (h - keys_at) * a.cache.stride_head
-                                           : static_cast<T*>(a.v_cache) + (h - values_at) * a.cache.stride_head);
-            } else {
-                continue;
-            }
-            *reinterpret_cast<R*>(dst + g0) = x[i][0];
-            *reinterpret_cast<R*>(dst + g1) = x[i][1];
+    // Queries go to q_out; keys and values to the token's cache row, if it has a block.
+    T* k_out = nullptr;
+    T* v_out = nullptr;
+    const int last = mine - (lane >> 4) + 2 * a.pairs_per_warp - 1;  // of the warp
+    if (last >= keys_at) {
+        int64_t row = 0;
+        if (tree_row(a.cache, b, span.base + t, &row)) {
+            k_out = static_cast<T*>(a.k_cache) + row;
+            v_out = static_cast<T*>(a.v_cache) + row;
+        } else if (lane == 0) {
+            raise_bad_input(a.cache.status);
         }
+    }
+    T* q_out = static_cast<T*>(a.q_out) + bt * a.q_out_stride;
+    __syncthreads();
+    if (mine - (lane >> 4) >= end) return;
+
+    // Coefficients of the lane's four pairs with the norm's weights in them, for queries or keys:
+    // y_a = v_a ca - v_c sc, y_c = v_a sa + v_c cc. Channels that are not rotated turn by nothing.
+    float ca[4], sa[4], sc[4], cc[4];
+    auto coefficients = [&](bool for_q) {
+        float wa[4] = {1.0f, 1.0f, 1.0f, 1.0f}, wc[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        if (NORM) {
+            const float* w = s_weight + (for_q ? 0 : kHeadDim);
+            const float4 w0 = *reinterpret_cast<const float4*>(w + g0);
+            const float4 w1 = *reinterpret_cast<const float4*>(w + g1);
+            if (HALF) {
+                wa[0] = w0.x; wa[1] = w0.y; wa[2] = w0.z; wa[3] = w0.w;
+                wc[0] = w1.x; wc[1] = w1.y; wc[2] = w1.z; wc[3] = w1.w;
+            } else {
+                wa[0] = w0.x; wa[1] = w0.z; wa[2] = w1.x; wa[3] = w1.z;
+                wc[0] = w0.y; wc[1] = w0.w; wc[2] = w1.y; wc[3] = w1.w;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float cs = rotated ? s_cos[4 * l + i] : 1.0f, sn = rotated ? s_sin[4 * l + i] : 0.0f;
+            ca[i] = cs * wa[i];
+            sa[i] = sn * wa[i];
+            sc[i] = sn * wc[i];
+            cc[i] = cs * wc[i];
+        }
+    };
+    bool for_q = mine < keys_at;
+    coefficients(for_q);
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        if (i >= a.pairs_per_warp) break;
+        const int h = mine + 2 * i;
+        float scale = 1.0f;
+        float v[2][4];
+        unpack(x[i][0], v[0]);
+        unpack(x[i][1], v[1]);
+        if (NORM) {
+            // Both halves of the warp take part, whatever their heads are.
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) sum += v[0][c] * v[0][c] + v[1][c] * v[1][c];
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            scale = rsqrtf(sum * (1.0f / kHeadDim) + a.eps);
+        }
+        if (h >= end) continue;
+        T* dst;
+        if (h < values_at) {
+            if (NORM && for_q != (h < keys_at)) {  // the first key behind queries
+                for_q = false;
+                coefficients(false);
+            }
+            float y[2][4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                // Pair c: channels g0 + c and g1 + c, or neighbours.
+                const int ga = HALF ? 0 : c >> 1, at = HALF ? c : 2 * (c & 1);
+                const int gc = HALF ? 1 : c >> 1, ct = HALF ? c : at + 1;
+                const float va = v[ga][at], vc = v[gc][ct];
+                y[ga][at] = va * ca[c] - vc * sc[c];
+                y[gc][ct] = va * sa[c] + vc * cc[c];
+                if (NORM) {
+                    y[ga][at] *= scale;
+                    y[gc][ct] *= scale;
+                }
+            }
+            pack(y[0], &x[i][0]);
+            pack(y[1], &x[i][1]);
+            dst = h < keys_at ? q_out + h * kHeadDim : k_out + (h - keys_at) * a.cache.stride_head;
+            if (h >= keys_at && k_out == nullptr) continue;
+        } else {
+            dst = v_out + (h - values_at) * a.cache.stride_head;
+            if (v_out == nullptr) continue;
+        }
+        *reinterpret_cast<R*>(dst + g0) = x[i][0];
+        *reinterpret_cast<R*>(dst + g1) = x[i][1];
     }
 }
 
 template <typename T>
-cudaError_t launch(const RopeArgs& a, int32_t nodes, bool half, dim3 grid, int threads, cudaStream_t stream) {
+cudaError_t launch(RopeArgs a, bool half, int32_t heads, int32_t sms, cudaStream_t stream) {
+    // kPairs pairs of heads per warp, so that angles and coefficients serve several, and a block per token
+    // where that is 8 warps at most; where the tokens alone do not fill the GPU (32 warps per SM) fewer
+    // pairs per warp, in blocks of two warps (the angles take 64 threads) that spread over the SMs.
+    const int64_t pairs = (heads + 1) / 2;
+    const int64_t share = (int64_t)a.batch * a.cache.tokens * pairs / ((int64_t)sms * 32);
+    a.pairs_per_warp = share < 1 ? 1 : (share > kPairs<T> ? kPairs<T> : (int32_t)share);
+    const int per_warp = 2 * a.pairs_per_warp;
+    int warps = (heads + per_warp - 1) / per_warp;
+    const int cols = a.pairs_per_warp == kPairs<T> ? (warps + kMaxWarps - 1) / kMaxWarps : (warps + 1) / 2;
+    warps = (warps + cols - 1) / cols;
+    warps = warps < 2 ? 2 : warps;
+    a.heads_per_block = warps * per_warp;
+    const dim3 grid((unsigned)((heads + a.heads_per_block - 1) / a.heads_per_block), (unsigned)a.cache.tokens,
+                    (unsigned)a.batch);
     auto kernel = half ? (a.weight != nullptr ? rope_append_kernel<T, true, true>
                                               : rope_append_kernel<T, true, false>)
                        : (a.weight != nullptr ? rope_append_kernel<T, false, true>
                                               : rope_append_kernel<T, false, false>);
-    return launch_pdl(kernel, grid, dim3((unsigned)threads), 0, stream, a, nodes);
+    return launch_pdl(kernel, grid, dim3((unsigned)warps * 32), 0, stream, a);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -270,28 +305,12 @@ extern "C" int gqa_rope_append(const gqa_rope_params* p) {
     a.attn_factor = p->attn_factor;
     int32_t sms = 0;
     if (current_sm_count(&sms) != GQA_OK) return GQA_ERR_CUDA;
-    const int64_t nodes = (int64_t)p->batch * p->tokens;
+    if (p->batch > 65535) return GQA_ERR_SHAPE;
+    a.batch = p->batch;
     const int32_t heads = p->num_q_heads + 2 * p->num_kv_heads;
-    // Up to kBatch pairs of heads per warp and 16 warps per block, i.e. a block per token for up to 128 heads;
-    // where the tokens alone do not fill the GPU (32 warps per SM) they are cut by heads, down to a pair
-    // per warp, in blocks of four warps that spread over the SMs.
-    const int64_t pairs = (heads + 1) / 2;
-    int64_t per_warp = nodes * pairs / ((int64_t)sms * 32);
-    per_warp = per_warp < 1 ? 1 : (per_warp > kBatch ? kBatch : per_warp);
-    int64_t warps = (pairs + per_warp - 1) / per_warp;
-    int64_t cols = per_warp < kBatch ? (warps + 3) / 4 : (warps + kMaxWarps - 1) / kMaxWarps;
-    if (cols * kMaxWarps < warps) cols = (warps + kMaxWarps - 1) / kMaxWarps;
-    warps = (warps + cols - 1) / cols;
-    a.heads_per_block = (int32_t)(2 * ((pairs + cols - 1) / cols));
-    cols = (heads + a.heads_per_block - 1) / a.heads_per_block;
-    warps = warps < 2 ? 2 : warps;  // the angles take 64 threads
-    const int64_t gy = nodes < 32768 ? nodes : 32768, gz = (nodes + gy - 1) / gy;
-    if (gz > 65535) return GQA_ERR_SHAPE;
-    const dim3 grid((unsigned)cols, (unsigned)gy, (unsigned)gz);
     cudaStream_t stream = reinterpret_cast<cudaStream_t>(p->stream);
     const bool half = p->style == GQA_ROPE_HALF;
-    const cudaError_t e = p->dtype == GQA_DTYPE_F32
-                              ? launch<float>(a, (int32_t)nodes, half, grid, (int)warps * 32, stream)
-                              : launch<__nv_bfloat16>(a, (int32_t)nodes, half, grid, (int)warps * 32, stream);
+    const cudaError_t e = p->dtype == GQA_DTYPE_F32 ? launch<float>(a, half, heads, sms, stream)
+                                                    : launch<__nv_bfloat16>(a, half, heads, sms, stream);
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
