@@ -946,12 +946,13 @@ def _on_device(name: str, t: torch.Tensor, dtype, home: int) -> int:
 
 
 def _token_rows(name: str, t: torch.Tensor, dtype, home: int):
-    """Address and token stride of [batch, tokens, heads, 128] rows whose tokens may lie apart."""
+    """Address and token stride (0: packed) of [batch, tokens, heads, 128] rows whose tokens may lie
+    apart."""
     if t.dtype is not dtype or t.get_device() != home:
         _refuse(name, t, dtype, None, home)
-    batch, tokens, heads, dim = t.shape
     if t.is_contiguous():
-        return t.data_ptr(), heads * dim
+        return t.data_ptr(), 0  # packed
+    batch, tokens, heads, dim = t.shape
     sb, st, sh, sd = t.stride()
     if tokens == 1:
         st = sb

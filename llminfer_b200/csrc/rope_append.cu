@@ -82,7 +82,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) rope_append_kernel(const Ro
     __shared__ float s_weight[NORM ? 2 * kHeadDim : 1];
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
-    const int warps = blockDim.x >> 5;
     const int heads = a.num_q_heads + 2 * a.num_kv_heads;
     const int keys_at = a.num_q_heads, values_at = a.num_q_heads + a.num_kv_heads;
     const int b = blockIdx.z, t = blockIdx.y;

@@ -72,7 +72,35 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile
     }
 }
 
-// The same by a whole warp: one answer, and the lanes together again.
+// Two FP32 numbers in one 64-bit register, and arithmetic on both at once: the weights' loop is bound by the
+// instructions a warp issues (a polynomial in place of some of its exponentials made it slower).
+struct Two {
+    uint64_t v;
+};
+__device__ __forceinline__ Two two_of(uint32_t lo, uint32_t hi) {
+    Two t;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "r"(lo), "r"(hi));
+    return t;
+}
+__device__ __forceinline__ Two two_of(float lo, float hi) { return two_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ void split(Two t, float* lo, float* hi) {
+    uint32_t a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(t.v));
+    *lo = __uint_as_float(a);
+    *hi = __uint_as_float(b);
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+
+// wait_bar by a whole warp: one answer, and the lanes together again.
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
     return __all_sync(0xffffffffu, wait_bar(bar, parity, dead));
 }
@@ -576,7 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_loaded(s[1]);
                         float top[4] = {mx, mx, mx, mx};
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[i >> 5][i & 31]));
+                        for (int i = 0; i < 32; ++i) {
+                            top[i & 3] = fmaxf(top[i & 3], fmaxf(__uint_as_float(s[0][i]), __uint_as_float(s[1][i])));
+                        }
                         mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                     }
                     if (j < 2) {
@@ -604,7 +634,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const float off = safe_max(m) * scale;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const Two factor = two_of(scale, scale), minus = two_of(-off, -off);
+                    Two sum[2] = {two_of(0.0f, 0.0f), two_of(0.0f, 0.0f)};
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
                         uint32_t s[2][32], w[32];
@@ -614,14 +645,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_loaded(s[1]);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const float e0 = ex2_approx(__uint_as_float(s[i >> 4][2 * i & 31]) * scale - off);
-                            const float e1 = ex2_approx(__uint_as_float(s[i >> 4][(2 * i & 31) + 1]) * scale - off);
-                            sum[i & 3] += e0 + e1;
+                            float e0, e1;
+                            split(fma2(two_of(s[i >> 4][2 * i & 31], s[i >> 4][(2 * i & 31) + 1]), factor, minus), &e0, &e1);
+                            e0 = ex2_approx(e0);
+                            e1 = ex2_approx(e1);
+                            sum[i & 1] = add2(sum[i & 1], two_of(e0, e1));
                             w[i] = pack_bf16(e0, e1);
                         }
                         tmem_store32(my_s + 32 * half, w);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    float l0, l1;
+                    split(add2(sum[0], sum[1]), &l0, &l1);
+                    l += l0 + l1;
                     tmem_stored();
                 }
                 tc_fence_before();
