@@ -5,6 +5,7 @@ the C++ shim in ``shim/`` that keeps the reference's operator interface. This Py
 is the thin binding used by the tests and the benchmark; it has no CPU fallback.
 """
 from .binding import (  # noqa: F401
+    DraftTree,
     FusedFront,
     SPLIT_EVEN,
     GqaError,

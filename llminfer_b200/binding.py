@@ -1138,3 +1138,62 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: i
         _want("tree_sizes", tree_sizes, torch.int32, (batch,), home), table,
         _want("seq_lens_out", seq_lens_out, torch.int32, (batch,), home),
         _want("status", status, torch.int32, None, home), _stream(stream, home))), "gqa_tree_commit")
+
+
+class DraftTree:
+    """The drafted trees of a batch on the device, and the four calls of a step on them.
+
+    plan() takes the trees' shapes and the histories; append() and attend() run per layer, then
+    verify() and commit() once, after which `history` holds the new lengths (on the device, ready for the
+    next plan()). All buffers are made here: a step after plan() allocates nothing and can be captured
+    in a graph; one object serves one stream at a time."""
+
+    def __init__(self, batch: int, tokens: int, num_q_heads: int, num_kv_heads: int, device="cuda",
+                 dtype: torch.dtype = torch.bfloat16):
+        self.batch, self.tokens, self.num_kv_heads = batch, tokens, num_kv_heads
+
+        def ints(*shape):
+            return torch.zeros(shape, dtype=torch.int32, device=device)
+
+        self.mask, self.depth = ints(batch, tokens, (tokens + 31) // 32), ints(batch, tokens)
+        self.parents, self.sizes = ints(batch, tokens), ints(batch)
+        self.lens, self.history = ints(batch), ints(batch)
+        self.path, self.kept, self.next_token = ints(batch, tokens), ints(batch), ints(batch)
+        self.status = ints(1)
+        self.workspace = tree_workspace(batch, tokens, num_q_heads, num_kv_heads, device, dtype)
+
+    def plan(self, parents: torch.Tensor, sizes: Optional[torch.Tensor] = None,
+             history: Optional[torch.Tensor] = None) -> None:
+        """parents [batch, tokens] and sizes [batch] on the host; history [batch]: cached positions in
+        front of the trees (None: what the last commit() left)."""
+        if sizes is None:
+            sizes = torch.full((self.batch,), self.tokens, dtype=torch.int32)
+        if tuple(parents.shape) != (self.batch, self.tokens):
+            raise ValueError(f"parents: shape {tuple(parents.shape)}, expected {(self.batch, self.tokens)}")
+        mask, depth = tree_masks(parents, sizes)
+        self.mask.copy_(mask, non_blocking=True)
+        self.depth.copy_(depth, non_blocking=True)
+        self.parents.copy_(parents, non_blocking=True)
+        self.sizes.copy_(sizes, non_blocking=True)
+        if history is not None:
+            self.history.copy_(history, non_blocking=True)
+        torch.add(self.history, self.sizes, out=self.lens)
+
+    def append(self, q, k_new, v_new, k_cache, v_cache, *, layout: KvLayout, freq, **kw) -> None:
+        rope_append(q, k_new, v_new, k_cache, v_cache, layout=layout, freq=freq, seq_lens_dev=self.lens,
+                    depth=self.depth, tree_sizes=self.sizes, status=self.status, **kw)
+
+    def attend(self, q, k_cache, v_cache, out, *, layout: KvLayout, **kw) -> None:
+        tree_decode(q, k_cache, v_cache, out, num_kv_heads=self.num_kv_heads, layout=layout,
+                    seq_lens_dev=self.lens, mask=self.mask, tree_sizes=self.sizes,
+                    workspace=self.workspace, status=self.status, **kw)
+
+    def verify(self, target, draft, tokens, u_accept, u_sample, **kw) -> None:
+        tree_verify(target, draft, tokens, self.parents, u_accept, u_sample, path=self.path,
+                    kept=self.kept, next_token=self.next_token, tree_sizes=self.sizes,
+                    status=self.status, **kw)
+
+    def commit(self, k_cache, v_cache, *, layout: KvLayout, layers: int = 1, **kw) -> None:
+        tree_commit(k_cache, v_cache, num_kv_heads=self.num_kv_heads, layout=layout, layers=layers,
+                    seq_lens_dev=self.lens, path=self.path, kept=self.kept, seq_lens_out=self.history,
+                    tree_sizes=self.sizes, status=self.status, **kw)

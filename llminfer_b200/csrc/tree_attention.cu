@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tok = key;
                         blk = a.cache.fixed_block;
                         if (a.cache.block_table != nullptr) {
-                            const int lb = fast_div(key, a.cache.block_tokens);
+                            const int lb = (int)((uint32_t)key / (uint32_t)a.cache.block_tokens);
                             tok = key - lb * a.cache.block_tokens;
                             blk = __ldg(a.cache.block_table + (int64_t)p.u.b * a.cache.blocks_per_seq + lb);
                             if ((uint32_t)blk >= (uint32_t)a.cache.num_blocks) {

@@ -516,6 +516,25 @@ def test_verify_edges(gqa):
     assert got[2][8] == 5 and got[2][10] == 60 and got[2][11] == -1
 
 
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_verify_of_many_sequences_over_a_large_vocabulary(gqa, with_draft):
+    """So many sequences that each gets one block, and more rounds of a warp's segment than are kept
+    (64 of 32 vectors): samples among the first rounds, the last ones, and a threshold nothing passes."""
+    gen = torch.Generator().manual_seed(12)
+    batch, nodes, vocab = 150, 2, 140001
+    target = torch.softmax(2.0 * torch.randn(batch, nodes, vocab, generator=gen), -1)
+    draft = torch.softmax(2.0 * torch.randn(batch, nodes, vocab, generator=gen), -1) if with_draft else None
+    parents = torch.tensor([[-1, 0]] * batch, dtype=torch.int32)
+    tokens = torch.randint(0, vocab, (batch, nodes), generator=gen).int()
+    u, us = torch.rand(batch, nodes, generator=gen), torch.rand(batch, generator=gen)
+    us[0], us[1], us[2] = 0.0, 1.0 - 2.0 ** -24, 1.0
+    got = run_verify(gqa, target.to(DEV), None if draft is None else draft.to(DEV), tokens, parents, u, us, [nodes] * batch)
+    for b in range(batch):
+        path, nxt = TH.verify(target[b], None if draft is None else draft[b], tokens[b].tolist(), parents[b].tolist(), nodes,
+                              u[b].double().tolist(), float(us[b].double()))
+        assert got[0][b][: len(path)] == path and got[1][b] == len(path) and got[2][b] == nxt, b
+
+
 def test_verify_emits_tokens_as_the_target_would(gqa):
     """The first token behind the root, accepted or sampled, over many seeded draws of two drafts from the
     draft's row: its frequencies are the target's, to five standard deviations of a count."""
@@ -690,3 +709,51 @@ def test_decode_loop(gqa, captured):
                     blk, at = int(table[b, p // block]), p % block
                     assert torch.equal(k[layer, blk, :, at], plain_k[layer, blk, :, at])
                     assert torch.equal(v[layer, blk, :, at], plain_v[layer, blk, :, at])
+
+
+def test_draft_tree_runs_the_four_calls(gqa):
+    """DraftTree is the four calls on buffers of its own: the same bits, and the next plan starts from
+    the lengths the last commit left."""
+    gen = torch.Generator().manual_seed(41)
+    hq, hkv, tokens, batch, vocab = 16, 4, 10, 2, 40
+    layout = gqa.layout_pool(8, 64, hkv)
+    table = ints([[0, 1, 2, 3], [4, 5, 6, 7]])
+    freq, factor = gqa.rope_frequencies(128)
+    freq = freq.to(DEV)
+    trees = torch.tensor([[-1, 0, 0, 1, 1, 2, 3, 3, 4, 5], [-1, 0, 1, 2, 3, 4, 5, 6, 7, 8]])
+    sizes, history = torch.tensor([10, 7]), torch.tensor([60, 100])
+    start = [torch.randn(8, hkv, 64, D, generator=gen).to(BF16).to(DEV) for _ in range(2)]
+    tree = gqa.DraftTree(batch, tokens, hq, hkv, DEV)
+    plain = [c.clone() for c in start]
+    own = [c.clone() for c in start]
+    for turn in range(2):
+        q, kn, vn = (torch.randn(batch, tokens, h, D, generator=gen).to(BF16).to(DEV) for h in (hq, hkv, hkv))
+        target = probabilities(gen, (batch, tokens, vocab), F32, 1.0).to(DEV)
+        draft = (0.9 * target + 0.1 / vocab)
+        words = torch.randint(0, vocab, (batch, tokens), generator=gen).int().to(DEV)
+        u, us = torch.rand(batch, tokens, generator=gen).to(DEV), torch.rand(batch, generator=gen).to(DEV)
+        tree.plan(trees, sizes, history if turn == 0 else None)
+        rot, out = torch.zeros_like(q), torch.zeros_like(q)
+        tree.append(q, kn, vn, own[0], own[1], layout=layout, freq=freq, attn_factor=factor, q_out=rot, block_table=table)
+        tree.attend(rot, own[0], own[1], out, layout=layout, block_table=table)
+        tree.verify(target, draft, words, u, us)
+        tree.commit(own[0], own[1], layout=layout, block_table=table)
+        lens = ints([int(h) + int(s) for h, s in zip(history, sizes)])
+        mask, depth = gqa.tree_masks(trees, sizes)
+        rot2, out2 = torch.zeros_like(q), torch.zeros_like(q)
+        ws = gqa.tree_workspace(batch, tokens, hq, hkv, DEV)
+        gqa.rope_append(q, kn, vn, plain[0], plain[1], layout=layout, seq_lens_dev=lens, freq=freq, attn_factor=factor, q_out=rot2,
+                        depth=depth.to(DEV), tree_sizes=ints(sizes.tolist()), block_table=table)
+        gqa.tree_decode(rot2, plain[0], plain[1], out2, num_kv_heads=hkv, layout=layout, seq_lens_dev=lens, mask=mask.to(DEV),
+                        tree_sizes=ints(sizes.tolist()), block_table=table, workspace=ws)
+        path, kept, nxt, new = ints([[0] * tokens] * batch), ints([0] * batch), ints([0] * batch), ints([0] * batch)
+        gqa.tree_verify(target, draft, words, trees.int().to(DEV), u, us, path=path, kept=kept, next_token=nxt, tree_sizes=ints(sizes.tolist()))
+        gqa.tree_commit(plain[0], plain[1], num_kv_heads=hkv, layout=layout, seq_lens_dev=lens, path=path, kept=kept, seq_lens_out=new,
+                        tree_sizes=ints(sizes.tolist()), block_table=table)
+        assert int(tree.status) == 0
+        for a, b in ((rot, rot2), (out, out2), (own[0], plain[0]), (own[1], plain[1]), (tree.path, path), (tree.kept, kept),
+                     (tree.next_token, nxt), (tree.history, new)):
+            assert torch.equal(a, b)
+        history = new.cpu()
+    with pytest.raises(ValueError, match="parents"):
+        tree.plan(trees[:, :5])
