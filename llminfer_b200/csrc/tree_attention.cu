@@ -181,7 +181,8 @@ __device__ void build_tables(const TreeArgs& a, const Tables& t) {
 }
 
 // The places cut over the CTAs: the first `extra` take per + 1 places, the others per; no more CTAs take
-// part than get two places each (one tile for each stream: fewer records to merge). 32-bit arithmetic: every role does this before its first instruction of use.
+// part than get two places each (one tile for each stream: fewer records to merge). 32-bit arithmetic: every
+// role does this before its first instruction of use.
 struct Cut {
     int total;
     int ctas;
@@ -317,7 +318,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         prefetch_tensormap(&map_v);
     }
     if (warp == 9) tmem_alloc(smem_u32(&s_tmem), kColumns);
-    for (int i = threadIdx.x; i < QT * kTileBytes / 16; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < QT * kTileBytes / 16; i += kThreads) {
+        reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    }
     fence_proxy_async();
     const int row_token = (threadIdx.x & 127) / a.group;  // of a softmax thread's row, inside its tile
     const int row_head = (threadIdx.x & 127) - row_token * a.group;
@@ -569,7 +572,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 clear = clear || (e[c] & 0x7f80u) == 0x7f80u || (e[c] & 0x7f800000u) == 0x7f800000u;
                             }
                         }
-                        if (clear) atomicOr(&s_bad[turn & 1][(key - base) >> 5], 1u << ((key - base) & 31));
+                        // With two query tiles the other stream looks over the same row and may have zeroed part of it
+                        // already: it names the row first, so a reader of its zeros finds the name.
+                        uint32_t* named = &s_bad[turn & 1][(key - base) >> 5];
+                        const uint32_t bit = 1u << ((key - base) & 31);
+                        if (clear) {
+                            atomicOr(named, bit);
+                            __threadfence_block();
+                        } else if (two) {
+                            __threadfence_block();
+                            clear = (*reinterpret_cast<volatile uint32_t*>(named) & bit) != 0;
+                        }
                     }
                     if (clear) {
 #pragma unroll 1
