@@ -100,7 +100,11 @@ extern "C" int gqa_tree_commit(const gqa_tree_commit_params* p) {
     if (p->path == nullptr || p->kept == nullptr || p->seq_lens_out == nullptr) return GQA_ERR_NULL;
     if (p->num_layers <= 0 || p->num_layers > 65535 || p->batch > 65535) return GQA_ERR_SHAPE;
     if (p->num_layers > 1 && p->layer_stride <= 0) return GQA_ERR_SHAPE;
-    if (p->seq_lens_out == p->seq_lens_dev) return GQA_ERR_UNSUPPORTED;
+    // One block of a sequence writes its length while the others still read these.
+    if (p->seq_lens_out == p->seq_lens_dev || p->seq_lens_out == p->kept || p->seq_lens_out == p->tree_sizes_dev ||
+        p->seq_lens_out == p->path) {
+        return GQA_ERR_UNSUPPORTED;
+    }
     a.elem_bytes = p->dtype == GQA_DTYPE_F32 ? 4 : 2;
     a.layer_bytes = p->layer_stride * a.elem_bytes;
     if (a.layer_bytes % 16 != 0) return GQA_ERR_ALIGN;

@@ -248,3 +248,11 @@ def test_binding_refuses_wrong_tensors(monkeypatch, gqa):
     with pytest.raises(ValueError, match="contiguous"):
         gqa.tree_verify(torch.zeros(2, 4, 9), None, torch.zeros(4, 2, dtype=torch.int32).t(), lens, lens, lens,
                         path=lens, kept=lens, next_token=lens)
+
+
+@pytest.mark.parametrize("alias", ["kept", "path", "tree_sizes_dev"])
+def test_tree_commit_refuses_lengths_on_top_of_its_inputs(gqa, alias):
+    """Blocks of one launch read the inputs while another writes the lengths."""
+    from llminfer_b200 import binding as B
+    p = _fill(B._TreeCommitParams(), gqa, num_layers=1, seq_lens_out=0x3000, **{alias: 0x3000})
+    assert gqa.lib().gqa_tree_commit(C.byref(p)) == -8
