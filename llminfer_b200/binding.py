@@ -1127,11 +1127,16 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: i
     home = torch.cuda.current_device()
     batch, nodes = path.shape
     dtype = k_cache.dtype
+    if layer_stride is None:
+        if layers > 1 and not (k_cache.is_contiguous() and v_cache.is_contiguous()
+                               and k_cache.numel() == v_cache.numel() and k_cache.numel() % layers == 0):
+            raise ValueError("layer_stride: needed where the caches are not packed, equal and whole layers")
+        layer_stride = k_cache.numel() // max(layers, 1)
     table, per_seq = _table(block_table, batch, home)
     _check(lib().gqa_tree_commit(_TREE_COMMIT.pack(
         _dtype_code(k_cache), batch, nodes, num_kv_heads, 128, layers, per_seq, fixed_block,
         layout.block_tokens, layout.num_blocks, layout.stride_block, layout.stride_token, layout.stride_head,
-        k_cache.numel() // layers if layer_stride is None else layer_stride,
+        layer_stride,
         _on_device("k_cache", k_cache, dtype, home), _on_device("v_cache", v_cache, dtype, home),
         _want("path", path, torch.int32, (batch, nodes), home), _want("kept", kept, torch.int32, (batch,), home),
         _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home),

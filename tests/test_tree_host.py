@@ -256,3 +256,18 @@ def test_tree_commit_refuses_lengths_on_top_of_its_inputs(gqa, alias):
     from llminfer_b200 import binding as B
     p = _fill(B._TreeCommitParams(), gqa, num_layers=1, seq_lens_out=0x3000, **{alias: 0x3000})
     assert gqa.lib().gqa_tree_commit(C.byref(p)) == -8
+
+
+def test_commit_wants_a_stride_for_layers_that_are_not_packed(monkeypatch, gqa):
+    """Half of a cache that holds K and V side by side has its layers twice as far apart as its size says."""
+    from llminfer_b200 import binding as B
+    monkeypatch.setattr(B.torch.cuda, "current_device", lambda: -1)
+    both = torch.zeros(3, 2, 64 * 2 * 128, dtype=torch.bfloat16)
+    ints = torch.zeros(1, dtype=torch.int32)
+    kw = dict(num_kv_heads=2, layout=gqa.layout_reference(1, 64, 2), seq_lens_dev=ints, path=torch.zeros(1, 4, dtype=torch.int32),
+              kept=ints, seq_lens_out=ints)
+    for k, v, layers in ((both[:, 0], both[:, 1], 3), (both[:, 0].contiguous(), both[:, 1], 3), (both, both, 5)):
+        with pytest.raises(ValueError, match="layer_stride"):
+            gqa.tree_commit(k, v, layers=layers, **kw)
+    with pytest.raises(gqa.GqaError):  # no layers
+        gqa.tree_commit(both, both, layers=0, stream=0, **kw)
