@@ -1036,7 +1036,7 @@ def rope_append(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, k_cac
         fixed_block, eps, attn_factor, layout.block_tokens, layout.num_blocks, layout.stride_block,
         layout.stride_token, layout.stride_head, q_stride, out_stride, k_stride, v_stride, q_ptr, out_ptr,
         k_ptr, v_ptr, _want("qk_weight", qk_weight, dtype, (2 * dim,), home),
-        _want("freq", freq, torch.float64, None, home), _on_device("k_cache", k_cache, dtype, home),
+        _want("freq", freq, torch.float64, freq.shape[:1], home), _on_device("k_cache", k_cache, dtype, home),
         _on_device("v_cache", v_cache, dtype, home),
         _want("seq_lens_dev", seq_lens_dev, torch.int32, (batch,), home),
         _want("tree_sizes", tree_sizes, torch.int32, (batch,), home),

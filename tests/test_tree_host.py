@@ -271,3 +271,13 @@ def test_commit_wants_a_stride_for_layers_that_are_not_packed(monkeypatch, gqa):
             gqa.tree_commit(k, v, layers=layers, **kw)
     with pytest.raises(gqa.GqaError):  # no layers
         gqa.tree_commit(both, both, layers=0, stream=0, **kw)
+
+
+def test_rope_append_wants_a_row_of_frequencies(monkeypatch, gqa):
+    from llminfer_b200 import binding as B
+    monkeypatch.setattr(B.torch.cuda, "current_device", lambda: -1)
+    q = torch.zeros(1, 4, 4, 128)
+    lens = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="freq"):
+        gqa.rope_append(q, q, q, q, q, layout=gqa.layout_reference(1, 64, 4), seq_lens_dev=lens,
+                        freq=torch.zeros(8, 2, dtype=torch.float64))
