@@ -33,12 +33,13 @@ KERNEL_SOURCES = [
     "csrc/tree_host.cpp",
     "csrc/tree_decode.cu",
     "csrc/tree_attention.cu",
+    "csrc/tree_rows.cu",
     "csrc/tree_verify.cu",
     "csrc/tree_commit.cu",
 ]
 KERNEL_HEADERS = ["csrc/ptx.cuh", "csrc/work_map.cuh", "csrc/decode_kernels.cuh",
                   "csrc/peer_window.cuh", "csrc/front_math.cuh", "csrc/tree_common.cuh",
-                  "csrc/tree_attention.cuh", "csrc/tcgen05.cuh"]
+                  "csrc/tree_attention.cuh", "csrc/tree_cut.cuh", "csrc/tcgen05.cuh"]
 
 
 def _stale(output: Path, inputs: list[Path]) -> bool:
