@@ -4,11 +4,14 @@
 // holds them) against tiles of 64 keys, S = Q K^T, P = 2^(S - m) with a running maximum m and sum l per row,
 // O = O 2^(m' - m) + P V; all of it FP32, the scale and log2(e) multiplied into Q.
 //
-// Layout. 256 threads; thread (r, c) = (tid / 16, tid % 16) owns RT rows r RT .. and of them the scores of the keys
-// c, c + 16, c + 32, c + 48 and the output channels 4 c .. + 3 and 64 + 4 c .. + 3. A row's scores lie in 16 lanes of one
-// warp, so that maximum and P (through shared memory) stay inside the warp. Products are packed pairs of FP32
-// (over channels in S, over output channels in O). K and V tiles come by cp.async, two tiles deep; rows are
-// padded to 132 floats, which spreads 8 of them over all banks.
+// Layout. 8 warps; a warp owns RT rows, a lane of them the scores of the keys `lane` and lane + 32 and the output channels
+// 4 lane .. + 3. 512 bytes of K or V take four cycles to load from shared memory, the same 16 bytes of Q or P for
+// all lanes one or two, so a warp spans keys and channels and holds several rows. (Half warps of 16 keys with rows of
+// their own: 197 us instead of 171 for 8 nodes of 32 / 8 heads over 32768 keys, 910 instead of 953 for 64.)
+// Maximum and P stay inside the warp. Products are packed pairs of FP32 (over channels in S, over output
+// channels in O). K and V tiles come by cp.async, two tiles deep; rows are padded to 132 floats, which
+// spreads 8 of them over all banks. Bound by shared memory and its latency at two warps per scheduler: 64 nodes
+// over 32768 keys run at 36 TFLOP/s, half of what the FP32 units could do; 8 nodes at a quarter of the memory's rate.
 //
 // Work. The flat sequence of key tiles of all units, cut evenly over one CTA per SM, as for BF16.
 //
@@ -31,11 +34,10 @@ constexpr int kStages = 2;
 
 template <int RT>
 struct Shape {
-    static constexpr int kRows = 16 * RT;
-    static constexpr int kWeightPitch = kRows + 4;
+    static constexpr int kRows = 8 * RT;
     static constexpr int kQ = kRows * kPitch;
     static constexpr int kStage = 2 * kKeys * kPitch;  // K, then V
-    static constexpr int kWeights = kKeys * kWeightPitch;
+    static constexpr int kWeights = kKeys * kRows;  // [warp][key][row of the warp]
     static constexpr size_t kBytes = (size_t)(kQ + kStages * kStage + kWeights) * sizeof(float);
 };
 
@@ -57,40 +59,44 @@ __device__ __forceinline__ Four load_four(const float* p) {
     return Four{Two{u.x}, Two{u.y}};
 }
 
-// RT neighbouring floats.
-__device__ __forceinline__ void load_rows(const float* p, float (&x)[1]) { x[0] = *p; }
+// N neighbouring floats.
 __device__ __forceinline__ void load_rows(const float* p, float (&x)[2]) {
     const float2 u = *reinterpret_cast<const float2*>(p);
     x[0] = u.x; x[1] = u.y;
 }
-__device__ __forceinline__ void load_rows(const float* p, float (&x)[4]) {
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
+template <int N>
+__device__ __forceinline__ void load_rows(const float* p, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(p + i);
+        x[i] = u.x; x[i + 1] = u.y; x[i + 2] = u.z; x[i + 3] = u.w;
+    }
 }
-__device__ __forceinline__ void store_rows(float* p, const float (&x)[1]) { *p = x[0]; }
 __device__ __forceinline__ void store_rows(float* p, const float (&x)[2]) {
     *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
 }
-__device__ __forceinline__ void store_rows(float* p, const float (&x)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+template <int N>
+__device__ __forceinline__ void store_rows(float* p, const float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        *reinterpret_cast<float4*>(p + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+    }
 }
 
 // O += P V over the keys of a tile; MASKED: weights below zero are keys the row does not see.
 template <int RT, bool MASKED>
-__device__ __forceinline__ void add_values(const float* weights, const float* values, Two (&o)[RT][4]) {
+__device__ __forceinline__ void add_values(const float* weights, const float* values, Two (&o)[RT][2]) {
 #pragma unroll 8
     for (int key = 0; key < kKeys; ++key) {
-        const Four lo = load_four(values + key * kPitch), hi = load_four(values + key * kPitch + 64);
+        const Four v = load_four(values + key * kPitch);
         float w[RT];
-        load_rows(weights + key * Shape<RT>::kWeightPitch, w);
+        load_rows(weights + key * RT, w);
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             if (MASKED && w[i] < 0.0f) continue;
             const Two ww = two_of(w[i], w[i]);
-            o[i][0] = fma2(ww, lo.a, o[i][0]);
-            o[i][1] = fma2(ww, lo.b, o[i][1]);
-            o[i][2] = fma2(ww, hi.a, o[i][2]);
-            o[i][3] = fma2(ww, hi.b, o[i][3]);
+            o[i][0] = fma2(ww, v.a, o[i][0]);
+            o[i][1] = fma2(ww, v.b, o[i][1]);
         }
     }
 }
@@ -104,10 +110,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_rows_kernel(const TreeArgs a
     float* s_w = s_kv + kStages * S::kStage;
     const Tables tables = tables_at(reinterpret_cast<int32_t*>(s_w + S::kWeights), a.batch);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int r = tid >> 4, c = tid & 15;
     pdl_wait();
     pdl_launch_dependents();
     build_tables<1>(a, tables);
+    float* weights = s_w + warp * kKeys * RT;
     const Cut cut = cut_of(a, tables, 1);
     int pos = cut.begin(blockIdx.x);
     const int pos_end = cut.begin(blockIdx.x + 1);
@@ -160,13 +166,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_rows_kernel(const TreeArgs a
             *reinterpret_cast<float4*>(s_q + row * kPitch + d) = x;
         }
         float m[RT], l[RT];
-        Two o[RT][4];
+        Two o[RT][2];
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
             m[i] = -INFINITY;
             l[i] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[i][k] = two_of(0.0f, 0.0f);
+            for (int k = 0; k < 2; ++k) o[i][k] = two_of(0.0f, 0.0f);
         }
         for (int j = 0; j < steps; ++j) {
             if (j + 1 < steps) load(j + 1);
@@ -174,51 +180,51 @@ __global__ void __launch_bounds__(kThreads, 1) tree_rows_kernel(const TreeArgs a
             copies_wait_all_but_one();
             __syncthreads();
             const float* keys = s_kv + (j % kStages) * S::kStage;
-            const float* values = keys + kKeys * kPitch + 4 * c;
+            const float* values = keys + kKeys * kPitch + 4 * lane;
             const int key0 = key_first + j * kKeys;
             const bool tail = key0 + kKeys > base;
 
-            Two s2[RT][4];
+            Two s2[RT][2];
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) s2[i][k] = two_of(0.0f, 0.0f);
+                for (int k = 0; k < 2; ++k) s2[i][k] = two_of(0.0f, 0.0f);
             }
 #pragma unroll 4
             for (int d = 0; d < kHeadDim; d += 4) {
-                Four q[RT], k[4];
+                Four q[RT], k[2];
 #pragma unroll
-                for (int i = 0; i < RT; ++i) q[i] = load_four(s_q + (r * RT + i) * kPitch + d);
+                for (int i = 0; i < RT; ++i) q[i] = load_four(s_q + (warp * RT + i) * kPitch + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) k[i] = load_four(keys + (c + 16 * i) * kPitch + d);
+                for (int i = 0; i < 2; ++i) k[i] = load_four(keys + (lane + 32 * i) * kPitch + d);
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) s2[i][n] = fma2(q[i].b, k[n].b, fma2(q[i].a, k[n].a, s2[i][n]));
+                    for (int n = 0; n < 2; ++n) s2[i][n] = fma2(q[i].b, k[n].b, fma2(q[i].a, k[n].a, s2[i][n]));
                 }
             }
-            float w[4][RT];  // scores, then weights
+            float w[2][RT];  // scores, then weights
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int n = 0; n < 2; ++n) {
                     float lo, hi;
                     split(s2[i][n], &lo, &hi);
                     w[n][i] = lo + hi;
                 }
             }
-            uint32_t unseen = 0;  // bit 4 i + n
+            uint32_t unseen = 0;  // bit 2 i + n
             if (tail) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
-                    const int t = (r * RT + i) / a.group;
+                    const int t = (warp * RT + i) / a.group;
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const int key = key0 + c + 16 * n;
+                    for (int n = 0; n < 2; ++n) {
+                        const int key = key0 + lane + 32 * n;
                         const bool sees = t < p.u.tokens && key < p.u.len &&
                                           (key < base || tree_sees(a.mask, row0 + t, words, p.u.token0 + t, key - base));
                         if (!sees) {
-                            unseen |= 1u << (4 * i + n);
+                            unseen |= 1u << (2 * i + n);
                             w[n][i] = -INFINITY;
                         }
                     }
@@ -226,33 +232,32 @@ __global__ void __launch_bounds__(kThreads, 1) tree_rows_kernel(const TreeArgs a
             }
 #pragma unroll
             for (int i = 0; i < RT; ++i) {
-                float top = fmaxf(fmaxf(w[0][i], w[1][i]), fmaxf(w[2][i], w[3][i]));
+                float top = fmaxf(w[0][i], w[1][i]);
 #pragma unroll
-                for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                if (__any_sync(0xffffffffu, top > m[i])) {
-                    const float next = fmaxf(m[i], top);
-                    const float alpha = exp2f(m[i] - safe_max(next));
-                    m[i] = next;
+                for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                if (top > m[i]) {
+                    const float alpha = exp2f(m[i] - safe_max(top));
+                    m[i] = top;
                     l[i] *= alpha;
                     const Two f = two_of(alpha, alpha), zero = two_of(0.0f, 0.0f);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) o[i][k] = fma2(o[i][k], f, zero);
+                    for (int k = 0; k < 2; ++k) o[i][k] = fma2(o[i][k], f, zero);
                 }
                 const float ref = safe_max(m[i]);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int n = 0; n < 2; ++n) {
                     w[n][i] = exp2f(w[n][i] - ref);
                     l[i] += w[n][i];
-                    if (unseen >> (4 * i + n) & 1u) w[n][i] = -1.0f;
+                    if (unseen >> (2 * i + n) & 1u) w[n][i] = -1.0f;
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 4; ++n) store_rows(s_w + (c + 16 * n) * S::kWeightPitch + r * RT, w[n]);
+            for (int n = 0; n < 2; ++n) store_rows(weights + (lane + 32 * n) * RT, w[n]);
             __syncwarp();
             if (tail) {
-                add_values<RT, true>(s_w + r * RT, values, o);
+                add_values<RT, true>(weights, values, o);
             } else {
-                add_values<RT, false>(s_w + r * RT, values, o);
+                add_values<RT, false>(weights, values, o);
             }
             __syncthreads();
         }
@@ -260,25 +265,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_rows_kernel(const TreeArgs a
         float* rec = a.workspace + (int64_t)(2 * blockIdx.x + (p.tile == 0 ? 1 : 0)) * a.tile_rows * kRecordCols;
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
-            const int row = r * RT + i;
+            const int row = warp * RT + i;
             const int t = row / a.group, g = row - t * a.group;
             float sum = l[i];
 #pragma unroll
-            for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (t >= p.u.tokens) continue;
-            float x[8];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) split(o[i][k], &x[2 * k], &x[2 * k + 1]);
+            float4 x;
+            split(o[i][0], &x.x, &x.y);
+            split(o[i][1], &x.z, &x.w);
             if (p.whole) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                float* out = static_cast<float*>(a.out) +
-                             ((row0 + t) * a.num_q_heads + p.u.hk * a.group + g) * kHeadDim + 4 * c;
-                *reinterpret_cast<float4*>(out) = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-                *reinterpret_cast<float4*>(out + 64) = make_float4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+                *reinterpret_cast<float4*>(static_cast<float*>(a.out) +
+                                           ((row0 + t) * a.num_q_heads + p.u.hk * a.group + g) * kHeadDim + 4 * lane) =
+                    make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
             } else {
-                *reinterpret_cast<float4*>(rec + (c * a.tile_rows + row) * 4) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(rec + ((c + 16) * a.tile_rows + row) * 4) = make_float4(x[4], x[5], x[6], x[7]);
-                if (c == 0) {
+                *reinterpret_cast<float4*>(rec + (lane * a.tile_rows + row) * 4) = x;
+                if (lane == 0) {
                     rec[kHeadDim * a.tile_rows + row] = m[i];
                     rec[(kHeadDim + 1) * a.tile_rows + row] = sum;
                 }
@@ -337,7 +340,7 @@ int launch_tree_rows(TreeArgs a, int32_t sm_count, cudaStream_t stream) {
     const int64_t per_seq = (int64_t)(ceil_div(a.cache.capacity, kTile) + kUnitPad) * a.num_kv_heads *
                             ceil_div(a.cache.tokens, a.tile_tokens);
     if (per_seq * a.batch > (1 << 30)) return GQA_ERR_SHAPE;
-    return a.tile_rows == 16 ? launch<1>(a, stream) : a.tile_rows == 32 ? launch<2>(a, stream) : launch<4>(a, stream);
+    return a.tile_rows == 16 ? launch<2>(a, stream) : a.tile_rows == 32 ? launch<4>(a, stream) : launch<8>(a, stream);
 }
 
 }  // namespace gqa
