@@ -1,10 +1,11 @@
 /*
  * gqa_b200 — C ABI of the B200 (sm_100a) decode-phase grouped-query attention library.
  *
- * One hot path of the LLMInfer engine is provided here and nothing else: Qwen3 decode
+ * The hot path of the LLMInfer engine is provided here: Qwen3 decode
  * attention (one query token per sequence against a BF16 or FP32 KV cache), with the
- * QK-Norm + RoPE + KV-append stage in front of it, the KV block pool it reads from and the
- * KV-head-parallel partition across the GPUs of one node. Every entry point takes plain
+ * QK-Norm + RoPE + KV-append stage in front of it, the KV block pool it reads from, the
+ * KV-head-parallel partition across the GPUs of one node, and the operators of a decode step
+ * that drafts a tree of tokens per sequence. Every entry point takes plain
  * pointers and sizes, returns a status code, never aborts, never synchronises the device
  * (except where stated) and has NO CPU fallback: without a CUDA device the compute entry
  * points return GQA_ERR_CUDA.
