@@ -149,8 +149,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) rope_append_kernel(const Ro
     if (mine - (lane >> 4) >= end) return;
 
     // Coefficients of the lane's four pairs with the norm's weights in them, for queries or keys:
-    // y_a = v_a ca - v_c sc, y_c = v_a sa + v_c cc. Channels that are not rotated turn by nothing.
-    float ca[4], sa[4], sc[4], cc[4];
+    // y_a = v_a ca + v_c sc, y_c = v_a sa + v_c cc. Channels that are not rotated turn by nothing. Two pairs at once:
+    // packed arithmetic, since a large launch is bound by the instructions it issues.
+    Two ca[2], sa[2], sc[2], cc[2];
     auto coefficients = [&](bool for_q) {
         float wa[4] = {1.0f, 1.0f, 1.0f, 1.0f}, wc[4] = {1.0f, 1.0f, 1.0f, 1.0f};
         if (NORM) {
@@ -166,12 +167,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) rope_append_kernel(const Ro
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float cs = rotated ? s_cos[4 * l + i] : 1.0f, sn = rotated ? s_sin[4 * l + i] : 0.0f;
-            ca[i] = cs * wa[i];
-            sa[i] = sn * wa[i];
-            sc[i] = sn * wc[i];
-            cc[i] = cs * wc[i];
+        for (int i = 0; i < 4; i += 2) {
+            const float c0 = rotated ? s_cos[4 * l + i] : 1.0f, s0 = rotated ? s_sin[4 * l + i] : 0.0f;
+            const float c1 = rotated ? s_cos[4 * l + i + 1] : 1.0f, s1 = rotated ? s_sin[4 * l + i + 1] : 0.0f;
+            ca[i / 2] = two_of(c0 * wa[i], c1 * wa[i + 1]);
+            sa[i / 2] = two_of(s0 * wa[i], s1 * wa[i + 1]);
+            sc[i / 2] = two_of(-s0 * wc[i], -s1 * wc[i + 1]);
+            cc[i / 2] = two_of(c0 * wc[i], c1 * wc[i + 1]);
         }
     };
     bool for_q = mine < keys_at;
@@ -180,47 +182,63 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 3) rope_append_kernel(const Ro
     for (int i = 0; i < kBatch; ++i) {
         if (i >= a.pairs_per_warp) break;
         const int h = mine + 2 * i;
-        float scale = 1.0f;
-        float v[2][4];
-        unpack(x[i][0], v[0]);
-        unpack(x[i][1], v[1]);
-        if (NORM) {
-            // Both halves of the warp take part, whatever their heads are.
-            float sum = 0.0f;
+        if (h - (lane >> 4) < values_at) {  // the same for the warp: its lower head is rotated
+            float v[2][4];
+            unpack(x[i][0], v[0]);
+            unpack(x[i][1], v[1]);
+            // The pairs' members: channels g0 + c and g1 + c, or neighbours.
+            Two va[2], vc[2];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sum += v[0][c] * v[0][c] + v[1][c] * v[1][c];
+            for (int k = 0; k < 2; ++k) {
+                va[k] = HALF ? two_of(v[0][2 * k], v[0][2 * k + 1]) : two_of(v[k][0], v[k][2]);
+                vc[k] = HALF ? two_of(v[1][2 * k], v[1][2 * k + 1]) : two_of(v[k][1], v[k][3]);
+            }
+            float scale = 1.0f;
+            if (NORM) {
+                // Both halves of the warp take part, whatever their heads are.
+                const Two squares = fma2(va[0], va[0], fma2(va[1], va[1], fma2(vc[0], vc[0], mul2(vc[1], vc[1]))));
+                float lo, hi;
+                split(squares, &lo, &hi);
+                float sum = lo + hi;
 #pragma unroll
-            for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            scale = rsqrtf(sum * (1.0f / kHeadDim) + a.eps);
+                for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                scale = rsqrtf(sum * (1.0f / kHeadDim) + a.eps);
+                if (for_q != (h < keys_at)) {  // the first key behind queries
+                    for_q = false;
+                    coefficients(false);
+                }
+            }
+            if (h < values_at && h < end && (NORM || rotated)) {  // else as it came, infinities too
+                const Two both = two_of(scale, scale);
+                float y[2][4];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    Two ya = fma2(va[k], ca[k], mul2(vc[k], sc[k]));
+                    Two yc = fma2(va[k], sa[k], mul2(vc[k], cc[k]));
+                    if (NORM) {
+                        ya = mul2(ya, both);
+                        yc = mul2(yc, both);
+                    }
+                    if (HALF) {
+                        split(ya, &y[0][2 * k], &y[0][2 * k + 1]);
+                        split(yc, &y[1][2 * k], &y[1][2 * k + 1]);
+                    } else {
+                        split(ya, &y[k][0], &y[k][2]);
+                        split(yc, &y[k][1], &y[k][3]);
+                    }
+                }
+                pack(y[0], &x[i][0]);
+                pack(y[1], &x[i][1]);
+            }
         }
         if (h >= end) continue;
         T* dst;
-        if (h < values_at) {
-            if (NORM && for_q != (h < keys_at)) {  // the first key behind queries
-                for_q = false;
-                coefficients(false);
-            }
-            float y[2][4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                // Pair c: channels g0 + c and g1 + c, or neighbours.
-                const int ga = HALF ? 0 : c >> 1, at = HALF ? c : 2 * (c & 1);
-                const int gc = HALF ? 1 : c >> 1, ct = HALF ? c : at + 1;
-                const float va = v[ga][at], vc = v[gc][ct];
-                y[ga][at] = va * ca[c] - vc * sc[c];
-                y[gc][ct] = va * sa[c] + vc * cc[c];
-                if (NORM) {
-                    y[ga][at] *= scale;
-                    y[gc][ct] *= scale;
-                }
-            }
-            pack(y[0], &x[i][0]);
-            pack(y[1], &x[i][1]);
-            dst = h < keys_at ? q_out + h * kHeadDim : k_out + (h - keys_at) * a.cache.stride_head;
-            if (h >= keys_at && k_out == nullptr) continue;
+        if (h < keys_at) {
+            dst = q_out + h * kHeadDim;
         } else {
-            dst = v_out + (h - values_at) * a.cache.stride_head;
-            if (v_out == nullptr) continue;
+            const bool key = h < values_at;
+            dst = (key ? k_out : v_out) + (h - (key ? keys_at : values_at)) * a.cache.stride_head;
+            if (k_out == nullptr) continue;
         }
         *reinterpret_cast<R*>(dst + g0) = x[i][0];
         *reinterpret_cast<R*>(dst + g1) = x[i][1];

@@ -14,34 +14,6 @@ constexpr int kTile = 128;    // keys per place
 constexpr int kUnitPad = 1;   // places a unit counts on top of its tiles
 constexpr int kRecordCols = kHeadDim + 2;
 
-// Two FP32 numbers in one 64-bit register, and arithmetic on both at once: half the instructions where a loop is bound
-// by those a warp issues.
-struct Two {
-    uint64_t v;
-};
-__device__ __forceinline__ Two two_of(uint32_t lo, uint32_t hi) {
-    Two t;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "r"(lo), "r"(hi));
-    return t;
-}
-__device__ __forceinline__ Two two_of(float lo, float hi) { return two_of(__float_as_uint(lo), __float_as_uint(hi)); }
-__device__ __forceinline__ void split(Two t, float* lo, float* hi) {
-    uint32_t a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(t.v));
-    *lo = __uint_as_float(a);
-    *hi = __uint_as_float(b);
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    Two d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-    Two d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-
 // x / d for 0 <= x < 2^30, d > 0 and quotients below 2^21: every role divides a few times before its first
 // instruction of use, alone in its warp, where the general division is a chain of a hundred cycles.
 __device__ __forceinline__ int fast_div(int x, int d) {

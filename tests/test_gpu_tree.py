@@ -379,6 +379,28 @@ def test_rope_append(gqa, dtype, style, norm, rotary, scaling, hq, hkv, tokens, 
         assert torch.equal(dq[b, n:].cpu(), q[b, n:])
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("style", ["half", "interleaved"])
+def test_channels_that_are_not_rotated_pass_bit_for_bit(gqa, dtype, style):
+    """Infinities, NaN and negative zeros among them touch no other channel."""
+    gen = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(1, 3, h, D, generator=gen).to(dtype) for h in (5, 3, 3))
+    for rows in (q, k):
+        rows[..., 64:68] = torch.tensor([float("inf"), -0.0, float("nan"), 1.0], dtype=dtype)
+        rows[..., 120], rows[..., 121] = -float("inf"), -0.0
+    layout = gqa.layout_reference(1, 32, 3)
+    kc, vc = (torch.zeros(32 * 3 * D, dtype=dtype, device=DEV) for _ in range(2))
+    out = torch.zeros(1, 3, 5, D, dtype=dtype, device=DEV)
+    freq, _ = gqa.rope_frequencies(64, 1e4)
+    gqa.rope_append(q.to(DEV), k.to(DEV), v.to(DEV), kc, vc, layout=layout, seq_lens_dev=ints([10]), freq=freq.to(DEV),
+                    q_out=out, style=style)
+    kind = torch.int16 if dtype is BF16 else torch.int32
+    keys = kc.cpu().view(32, 3, D)[7:10]
+    assert torch.equal(out[0].cpu().view(kind)[..., 64:], q[0].view(kind)[..., 64:])
+    assert torch.equal(keys.view(kind)[..., 64:], k[0].view(kind)[..., 64:])
+    assert torch.isfinite(out[..., :64]).all() and torch.isfinite(keys[..., :64]).all()
+
+
 def test_rope_append_agrees_with_the_front_stage(gqa):
     """At near positions, rotate-half over the whole head with QK-Norm is what gqa_qk_norm_rope_append
     computes with FP32 angles: one unit in the last place of BF16."""
