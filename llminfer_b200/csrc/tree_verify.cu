@@ -17,7 +17,9 @@
 // same steps); after a pass the CTAs read one another's partial sums through distributed shared
 // memory. To place the sample, the partial sums name the segment in which the cumulative sum
 // passes u S, the kept sums of its rounds the round of 32 vectors, and one warp looks through that. A pass is bound by the latency of its loads: a lane
-// has eight vectors of each row in flight (two: 4.4 us a pass over 16000 elements per CTA).
+// has eight vectors of each row in flight (two: 4.4 us a pass over 16000 elements per CTA). Measured: 16 sequences of 32
+// nodes over 128000 words 21 us (up to four passes that depend on one another, about 3 us each, with 2 us of exchange and
+// walk), 64 sequences over 151643 words without draft probabilities 20 us, one of 8 nodes over 32768 words 7 us.
 #include <cuda_bf16.h>
 
 #include <cstring>
