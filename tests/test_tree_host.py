@@ -281,3 +281,9 @@ def test_rope_append_wants_a_row_of_frequencies(monkeypatch, gqa):
     with pytest.raises(ValueError, match="freq"):
         gqa.rope_append(q, q, q, q, q, layout=gqa.layout_reference(1, 64, 4), seq_lens_dev=lens,
                         freq=torch.zeros(8, 2, dtype=torch.float64))
+
+
+def test_tree_decode_refuses_output_on_top_of_the_queries(gqa):
+    from llminfer_b200 import binding as B
+    p = _fill(B._TreeDecodeParams(), gqa, workspace_bytes=1 << 40)
+    assert p.q == p.out and gqa.lib().gqa_tree_decode(C.byref(p)) == -8
