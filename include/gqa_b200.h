@@ -633,6 +633,9 @@ int gqa_qkv_gemv(const gqa_qkv_params* p);
  * Rows t >= n_b of per-node outputs are left as they were. A sequence whose length or size is out of
  * range (n_b < 0, n_b > tokens, seq_len < n_b, seq_len beyond what its blocks hold) is skipped and
  * *status_dev (optional) set to GQA_STATUS_BAD_INPUT. At most GQA_TREE_MAX_TOKENS nodes.
+ * The four wait for earlier work of the stream before they read anything, and may be captured in graphs.
+ * Behind them gqa_decode_params.early_prefetch is not to be set until the stream has been synchronised (or
+ * a launch of another library waited): they write lengths and rows of more than the newest position.
  */
 #define GQA_TREE_MAX_TOKENS 128
 
