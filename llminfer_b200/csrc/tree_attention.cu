@@ -26,7 +26,7 @@
 // NaN is zeroed too, and added by hand to the rows that see it, in the epilogue.
 //
 // Measured (32 / 8 heads unless stated): 16 sequences of 256 - 8192 keys, 16 nodes: 63 us, 4.5 TB/s; 64 nodes of 64 / 8
-// heads over 32768 keys: 89 us, 770 TFLOP/s, bound by the chain of a stream's products and weights; 8 nodes over 1024 keys: 11 us with the
+// heads over 32768 keys: 86 us, 800 TFLOP/s, bound by the chain of a stream's products and weights; 8 nodes over 1024 keys: 11 us with the
 // merge; 4 x 131072 keys, 64 / 8 heads, 8 nodes: 310 - 345 us in a short burst, 381 us at the clock of a long one.
 #include <cuda_bf16.h>
 
@@ -655,9 +655,7 @@ int launch(const TreeArgs& a, const CUtensorMap& mq, const CUtensorMap& mk, cons
     if (launch_pdl(kernel, dim3(a.ctas), dim3(kThreads), smem, stream, mq, mk, mv, a) != cudaSuccess) {
         return GQA_ERR_CUDA;
     }
-    const int unit_tokens = a.cache.tokens < a.tile_tokens * QT ? a.cache.tokens : a.tile_tokens * QT;
-    const dim3 grid((unsigned)a.ctas, (unsigned)ceil_div(unit_tokens * a.group, 8));
-    return launch_pdl(tree_merge_kernel<QT, __nv_bfloat16>, grid, dim3(256), 0, stream, a) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+    return launch_merge<QT, __nv_bfloat16>(a, stream) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
 }  // namespace

@@ -13,6 +13,8 @@ namespace {
 constexpr int kTile = 128;    // keys per place
 constexpr int kUnitPad = 1;   // places a unit counts on top of its tiles
 constexpr int kRecordCols = kHeadDim + 2;
+constexpr int kLongList = 30;  // records of a unit that a merge shares among its threads
+constexpr int kFewGroups = 8;  // groups of 8 rows up to which the merge has a block for every CTA
 
 // x / d for 0 <= x < 2^30, d > 0 and quotients below 2^21: every role divides a few times before its first
 // instruction of use, alone in its warp, where the general division is a chain of a hundred cycles.
@@ -154,42 +156,90 @@ __device__ __forceinline__ bool next_piece(const TreeArgs& a, const Tables& t, i
     return false;
 }
 
-// Merges the records of the units that were cut: out = sum_i O_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), pieces in
-// ascending order. grid.x: CTAs of the launch before, each of which starts at most one unit that others
-// finish and has left its description; grid.y: groups of 8 rows. Thread: row tid % 8 of the group, channels
-// 4 (tid / 8) .. + 3.
+// Merges the records of the units that were cut: out = sum_i O_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), in a fixed
+// order. grid.y: groups of 8 rows. grid.x: the CTAs of the launch before, each of which starts at most one unit that
+// others finish and has left its description; or, when there are fewer units than CTAs and many groups of rows, the
+// cut units, for which a block looks through all descriptions: blocks with nothing to do then took longer to
+// start than the others to merge (64 nodes of 64 / 8 heads over 32768 keys, 4736 blocks or 512: 91 or 86 us; with 64
+// rows the search costs more: 11.3 or 12.1 us for 8 nodes over 1024 keys). Thread: row tid % 8 of the group,
+// channels 4 (tid / 8 % 32) .. + 3, and of the unit's records those of its part of 256 threads: each record is a round
+// trip to L2, six at once, so that long lists (few units cut over all SMs) are shared by PARTS parts of a block.
 __device__ __forceinline__ void store4(__nv_bfloat16* p, float4 x) {
     *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
 }
 __device__ __forceinline__ void store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
 
-template <int QT, typename T>
-__global__ void __launch_bounds__(256, 4) tree_merge_kernel(const TreeArgs a) {
-    const int r = blockIdx.y * 8 + (threadIdx.x & 7);  // row of the unit
+template <int QT, typename T, int PARTS>
+__global__ void __launch_bounds__(256 * PARTS, 4 / PARTS) tree_merge_kernel(const TreeArgs a) {
+    __shared__ float4 s_o[PARTS > 1 ? PARTS - 1 : 1][256];
+    __shared__ float2 s_ml[PARTS > 1 ? PARTS - 1 : 1][256];
+    __shared__ int4 s_head;
+    __shared__ int s_count[8 * PARTS], s_tokens, s_c0;
+    const int part = threadIdx.x >> 8, tid = threadIdx.x & 255;
+    const int r = blockIdx.y * 8 + (tid & 7);  // row of the unit
     const int tile_rows = a.tile_tokens * a.group;
     const int tile = r >= tile_rows ? 1 : 0, row = r - tile * tile_rows;
-    const int chunk = threadIdx.x >> 3;
+    const int chunk = tid >> 3;
     const int token = r / a.group;  // of the unit
     const int64_t record = (int64_t)QT * a.tile_rows * kRecordCols;
     const float* rec = a.workspace + (int64_t)tile * a.tile_rows * kRecordCols;
-    const int c0 = blockIdx.x;
     T* out = static_cast<T*>(a.out) + (r - token * a.group) * kHeadDim + chunk * 4;
+    if (threadIdx.x == 0) s_c0 = -1;
     pdl_launch_dependents();
     pdl_wait();
-    const int4 head = __ldcg(a.cut_units + 2 * c0);  // last CTA, sequence, KV head, first token
-    const int c1 = head.x;
-    if (c1 < 0 || token >= __ldcg(a.cut_units + 2 * c0 + 1).x) return;
+    int c0 = blockIdx.x;
+    int4 head;  // last CTA, sequence, KV head, first token
+    int tokens;
+    if (PARTS == 1 && gridDim.x == (unsigned)a.ctas) {
+        head = __ldcg(a.cut_units + 2 * c0);
+        if (head.x < 0) return;
+        tokens = __ldcg(a.cut_units + 2 * c0 + 1).x;
+    } else {
+        int passed = 0;
+        for (int from = 0; from < a.ctas; from += 256 * PARTS) {
+            const int c = from + threadIdx.x, warp = threadIdx.x >> 5;
+            int4 one = make_int4(-1, 0, 0, 0);
+            int its_tokens = 0;
+            if (c < a.ctas) {
+                one = __ldcg(a.cut_units + 2 * c);
+                its_tokens = __ldcg(a.cut_units + 2 * c + 1).x;
+            }
+            const uint32_t cut = __ballot_sync(0xffffffffu, one.x >= 0);
+            if ((threadIdx.x & 31) == 0) s_count[warp] = __popc(cut);
+            __syncthreads();
+            int before = passed + __popc(cut & ((1u << (threadIdx.x & 31)) - 1u));
+            for (int w = 0; w < 8 * PARTS; ++w) {
+                before += w < warp ? s_count[w] : 0;
+                passed += s_count[w];
+            }
+            if (one.x >= 0 && before == (int)blockIdx.x) {
+                s_head = one;
+                s_tokens = its_tokens;
+                s_c0 = c;
+            }
+            __syncthreads();
+        }
+        c0 = s_c0;
+        if (c0 < 0) return;
+        head = s_head;
+        tokens = s_tokens;
+    }
+    const bool live = token < tokens;
+    if (PARTS == 1 && !live) return;
+    // The part's records: CTAs first .. last.
+    const int count = head.x - c0 + 1, share = ceil_div(count, PARTS);
+    const int first = c0 + part * share, last = live ? min(head.x, first + share - 1) : -1;
     auto at = [&](int c) { return rec + (int64_t)(2 * c + (c == c0 ? 1 : 0)) * record; };
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     constexpr int kBatch = 6;
-    for (int c = c0; c <= c1; c += kBatch) {
+    for (int c = first; c <= last; c += kBatch) {
         float mi[kBatch], li[kBatch];
         float4 oi[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             mi[i] = -INFINITY;
-            if (c + i > c1) continue;
+            if (c + i > last) continue;
             const float* p = at(c + i);
             mi[i] = __ldcg(p + kHeadDim * a.tile_rows + row);
             li[i] = __ldcg(p + (kHeadDim + 1) * a.tile_rows + row);
@@ -204,16 +254,54 @@ __global__ void __launch_bounds__(256, 4) tree_merge_kernel(const TreeArgs a) {
         o.x *= f; o.y *= f; o.z *= f; o.w *= f;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            if (c + i > c1) continue;
+            if (c + i > last) continue;
             const float w = ex2_approx(mi[i] - ref);
             l += li[i] * w;
             o.x += oi[i].x * w; o.y += oi[i].y * w; o.z += oi[i].z * w; o.w += oi[i].w * w;
         }
         m = next;
     }
+    if (PARTS > 1) {
+        if (part > 0) {
+            s_o[part - 1][tid] = o;
+            s_ml[part - 1][tid] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (part > 0 || !live) return;
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < PARTS - 1; ++i) top = fmaxf(top, s_ml[i][tid].x);
+        const float ref = safe_max(top);
+        const float f = ex2_approx(m - ref);
+        l *= f;
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+#pragma unroll
+        for (int i = 0; i < PARTS - 1; ++i) {
+            const float2 ml = s_ml[i][tid];
+            const float4 x = s_o[i][tid];
+            const float w = ex2_approx(ml.x - ref);
+            l += ml.y * w;
+            o.x += x.x * w; o.y += x.y * w; o.z += x.z * w; o.w += x.w * w;
+        }
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     out += (((int64_t)head.y * a.cache.tokens + head.w + token) * a.num_q_heads + head.z * a.group) * kHeadDim;
     store4(out, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+}
+
+// Units are at most batch * heads * runs; where the SMs are kLongList or more times as many, a unit has that many records
+// (one unit of 252 rows over 16486 keys: 27 us with four parts, 42 with one).
+template <int QT, typename T>
+cudaError_t launch_merge(const TreeArgs& a, cudaStream_t stream) {
+    const int unit = a.tile_tokens * QT;
+    const int unit_tokens = a.cache.tokens < unit ? a.cache.tokens : unit;
+    const int64_t units = (int64_t)a.batch * a.num_kv_heads * ceil_div(a.cache.tokens, unit);
+    const int groups = ceil_div(unit_tokens * a.group, 8);
+    const bool search = groups > kFewGroups && units < a.ctas;
+    const dim3 grid((unsigned)(search ? units : a.ctas), (unsigned)groups);
+    return search && units * kLongList <= a.ctas
+               ? launch_pdl(tree_merge_kernel<QT, T, 4>, grid, dim3(1024), 0, stream, a)
+               : launch_pdl(tree_merge_kernel<QT, T, 1>, grid, dim3(256), 0, stream, a);
 }
 
 }  // namespace

@@ -315,9 +315,7 @@ int launch(const TreeArgs& a, cudaStream_t stream) {
         }
     }
     if (launch_pdl(kernel, dim3(a.ctas), dim3(kThreads), smem, stream, a) != cudaSuccess) return GQA_ERR_CUDA;
-    const int unit_tokens = a.cache.tokens < a.tile_tokens ? a.cache.tokens : a.tile_tokens;
-    const dim3 grid((unsigned)a.ctas, (unsigned)ceil_div(unit_tokens * a.group, 8));
-    return launch_pdl(tree_merge_kernel<1, float>, grid, dim3(256), 0, stream, a) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
+    return launch_merge<1, float>(a, stream) == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
 
 size_t record_bytes(int32_t tokens, int32_t group, int32_t ctas) {

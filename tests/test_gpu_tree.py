@@ -97,6 +97,12 @@ def test_attention_over_a_long_history_cut_over_many_blocks(gqa, dtype):
     attend(gqa, 5, [6000], [12], 12, 8, 1, 0, dtype, "tree")
 
 
+@pytest.mark.parametrize("tokens,hq,hkv,length", [(36, 7, 1, 9001), (128, 8, 2, 5000), (33, 8, 1, 300)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_few_units_of_many_rows_merge_long_lists_of_pieces(gqa, tokens, hq, hkv, length, dtype):
+    attend(gqa, tokens, [length], [tokens], tokens, hq, hkv, 0, dtype, "random")
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_rows_that_see_nothing_are_zero(gqa, dtype):
     attend(gqa, 3, [6, 40], [6, 6], 6, 8, 2, 32, dtype, "none")
