@@ -25,9 +25,9 @@
 // rows past the end are zeroed in shared memory (0 * NaN). A node's V row that holds an infinity or
 // NaN is zeroed too, and added by hand to the rows that see it, in the epilogue.
 //
-// Measured (32 / 8 heads unless stated): 16 sequences of 256 - 8192 keys, 16 nodes: 63 us, 4.5 TB/s; 64 nodes of 64 / 8
+// Measured (32 / 8 heads unless stated): 16 sequences of 256 - 8192 keys, 16 nodes: 66 us, 4.5 TB/s; 64 nodes of 64 / 8
 // heads over 32768 keys: 86 us, 800 TFLOP/s, bound by the chain of a stream's products and weights; 8 nodes over 1024 keys: 11 us with the
-// merge; 4 x 131072 keys, 64 / 8 heads, 8 nodes: 310 - 345 us in a short burst, 381 us at the clock of a long one.
+// merge; 4 x 131072 keys, 64 / 8 heads, 8 nodes: 313 - 335 us in a short burst, 381 us at the clock of a long one.
 #include <cuda_bf16.h>
 
 #include <cstring>
