@@ -1170,7 +1170,8 @@ class DraftTree:
     def plan(self, parents: torch.Tensor, sizes: Optional[torch.Tensor] = None,
              history: Optional[torch.Tensor] = None) -> None:
         """parents [batch, tokens] and sizes [batch] on the host; history [batch]: cached positions in
-        front of the trees (None: what the last commit() left)."""
+        front of the trees (None: what the last commit() left). Host tensors are the caller's again when this
+        returns, pinned ones too, whatever the stream is still doing."""
         if sizes is None:
             sizes = torch.full((self.batch,), self.tokens, dtype=torch.int32)
         if tuple(parents.shape) != (self.batch, self.tokens):
@@ -1178,11 +1179,19 @@ class DraftTree:
         mask, depth = tree_masks(parents, sizes)
         self.mask.copy_(mask, non_blocking=True)
         self.depth.copy_(depth, non_blocking=True)
-        self.parents.copy_(parents, non_blocking=True)
-        self.sizes.copy_(sizes, non_blocking=True)
+        self._upload(self.parents, parents)
+        self._upload(self.sizes, sizes)
         if history is not None:
-            self.history.copy_(history, non_blocking=True)
+            self._upload(self.history, history)
         torch.add(self.history, self.sizes, out=self.lens)
+
+    @staticmethod
+    def _upload(to: torch.Tensor, values: torch.Tensor) -> None:
+        # A copy from pinned memory reads it when the stream gets there. A pageable copy of it is
+        # staged before the call returns and does not wait for the stream either.
+        if not values.is_cuda:
+            values = values.to(dtype=to.dtype, copy=True)
+        to.copy_(values, non_blocking=True)
 
     def append(self, q, k_new, v_new, k_cache, v_cache, *, layout: KvLayout, freq, **kw) -> None:
         rope_append(q, k_new, v_new, k_cache, v_cache, layout=layout, freq=freq, seq_lens_dev=self.lens,

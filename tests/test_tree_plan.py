@@ -1,0 +1,29 @@
+"""DraftTree.plan on the host: what it takes and what it leaves in the buffers."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def gqa(built_lib):
+    import llminfer_b200 as pkg
+    return pkg
+
+
+@pytest.fixture
+def tree(monkeypatch, gqa):
+    """A DraftTree of two sequences on the host: plan() needs no GPU."""
+    from llminfer_b200 import binding as B
+    monkeypatch.setattr(B, "tree_workspace", lambda *a: torch.zeros(16, dtype=torch.uint8))
+    return gqa.DraftTree(2, 4, 8, 2, "cpu")
+
+
+PARENTS = torch.tensor([[-1, 0, 0, 1], [-1, 0, 1, 2]])
+
+
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_plan_fills_the_buffers(tree, kind):
+    tree.plan(PARENTS.to(kind), torch.tensor([4, 2], dtype=kind), torch.tensor([5, 6], dtype=kind))
+    assert tree.lens.tolist() == [9, 8] and tree.history.tolist() == [5, 6] and tree.sizes.tolist() == [4, 2]
+    assert torch.equal(tree.parents, PARENTS.int())
+    tree.plan(PARENTS)  # from the lengths that are there
+    assert tree.lens.tolist() == [9, 10] and tree.sizes.tolist() == [4, 4]
