@@ -1176,6 +1176,11 @@ class DraftTree:
             sizes = torch.full((self.batch,), self.tokens, dtype=torch.int32)
         if tuple(parents.shape) != (self.batch, self.tokens):
             raise ValueError(f"parents: shape {tuple(parents.shape)}, expected {(self.batch, self.tokens)}")
+        if history is not None:
+            if tuple(history.shape) != (self.batch,):
+                raise ValueError(f"history: shape {tuple(history.shape)}, expected {(self.batch,)}")
+            if history.dtype.is_floating_point or history.dtype.is_complex or history.dtype == torch.bool:
+                raise TypeError(f"history: dtype {history.dtype}, expected whole numbers")
         mask, depth = tree_masks(parents, sizes)
         self.mask.copy_(mask, non_blocking=True)
         self.depth.copy_(depth, non_blocking=True)

@@ -20,6 +20,19 @@ def tree(monkeypatch, gqa):
 PARENTS = torch.tensor([[-1, 0, 0, 1], [-1, 0, 1, 2]])
 
 
+@pytest.mark.parametrize("history", [torch.tensor([5]), torch.tensor(5), torch.tensor([5, 6, 7]), torch.tensor([[5, 6]])])
+def test_plan_refuses_a_history_of_another_shape(tree, history):
+    """One number is not spread over all sequences."""
+    with pytest.raises(ValueError, match="history"):
+        tree.plan(PARENTS, None, history)
+
+
+@pytest.mark.parametrize("history", [torch.tensor([5.5, 6.0]), torch.tensor([True, False])])
+def test_plan_refuses_a_history_that_is_not_whole_numbers(tree, history):
+    with pytest.raises(TypeError, match="history"):
+        tree.plan(PARENTS, None, history)
+
+
 @pytest.mark.parametrize("kind", [torch.int32, torch.int64])
 def test_plan_fills_the_buffers(tree, kind):
     tree.plan(PARENTS.to(kind), torch.tensor([4, 2], dtype=kind), torch.tensor([5, 6], dtype=kind))
