@@ -820,7 +820,9 @@ int gqa_tree_verify(const gqa_tree_verify_params* p);
  * slot seq_len - n_b + i for i < kept[b], in place, and seq_lens_out[b] = seq_len - n_b + kept[b].
  * path must ascend (path[i] > path[i - 1], path[i] < n_b), as gqa_tree_verify leaves it; a sequence whose
  * path does not, or whose kept is outside 0 .. n_b, is skipped with its length unchanged
- * (GQA_STATUS_BAD_INPUT). Slots behind the kept rows are left as they are.
+ * (GQA_STATUS_BAD_INPUT): seq_lens_out[b] = seq_len, which still counts the nodes. A loop that takes
+ * seq_lens_out as the next step's history calls gqa_tree_commit_history, where a skipped sequence keeps
+ * its history instead. Slots behind the kept rows are left as they are.
  *   dtype            GQA_DTYPE_BF16 or GQA_DTYPE_F32 (rows are moved bit for bit).
  *   num_layers, layer_stride   the caches of layer l start l * layer_stride elements behind k_cache /
  *                    v_cache; layout and block table are the same for all layers.
@@ -851,6 +853,12 @@ typedef struct gqa_tree_commit_params {
 } gqa_tree_commit_params;
 
 int gqa_tree_commit(const gqa_tree_commit_params* p);
+
+/*
+ * gqa_tree_commit, but a sequence that is skipped leaves seq_lens_out[b] = seq_len - n_b: none of its nodes
+ * becomes history. (seq_len itself where n_b is outside 0 .. tokens or above seq_len.)
+ */
+int gqa_tree_commit_history(const gqa_tree_commit_params* p);
 
 #ifdef __cplusplus
 }

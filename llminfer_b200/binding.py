@@ -345,6 +345,7 @@ _SIGNATURES = {
     "gqa_tree_decode": (C.c_int, [C.c_void_p]),  # _TreeDecodeParams
     "gqa_tree_verify": (C.c_int, [C.c_void_p]),  # _TreeVerifyParams
     "gqa_tree_commit": (C.c_int, [C.c_void_p]),  # _TreeCommitParams
+    "gqa_tree_commit_history": (C.c_int, [C.c_void_p]),  # _TreeCommitParams
 }
 
 _lib: Optional[C.CDLL] = None
@@ -1120,10 +1121,13 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: i
                 kept: torch.Tensor, seq_lens_out: torch.Tensor, layers: int = 1,
                 layer_stride: Optional[int] = None, tree_sizes: Optional[torch.Tensor] = None,
                 block_table: Optional[torch.Tensor] = None, fixed_block: int = 0,
-                status: Optional[torch.Tensor] = None, stream: Optional[int] = None) -> None:
+                status: Optional[torch.Tensor] = None, stream: Optional[int] = None,
+                keep_history: bool = False) -> None:
     """Moves the accepted path's K and V rows to the first of the draft's cache slots in `layers`
     caches that lie layer_stride elements apart (default: the tensors cut in `layers` equal parts)
-    and leaves the new lengths in seq_lens_out (another tensor than seq_lens_dev)."""
+    and leaves the new lengths in seq_lens_out (another tensor than seq_lens_dev). A sequence that is
+    skipped (see `status`) leaves its seq_lens_dev there, drafted nodes and all, or with keep_history
+    its history alone."""
     home = torch.cuda.current_device()
     batch, nodes = path.shape
     dtype = k_cache.dtype
@@ -1133,7 +1137,8 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, *, num_kv_heads: i
             raise ValueError("layer_stride: needed where the caches are not packed, equal and whole layers")
         layer_stride = k_cache.numel() // max(layers, 1)
     table, per_seq = _table(block_table, batch, home)
-    _check(lib().gqa_tree_commit(_TREE_COMMIT.pack(
+    call = lib().gqa_tree_commit_history if keep_history else lib().gqa_tree_commit
+    _check(call(_TREE_COMMIT.pack(
         _dtype_code(k_cache), batch, nodes, num_kv_heads, 128, layers, per_seq, fixed_block,
         layout.block_tokens, layout.num_blocks, layout.stride_block, layout.stride_token, layout.stride_head,
         layer_stride,
@@ -1150,8 +1155,9 @@ class DraftTree:
 
     plan() takes the trees' shapes and the histories; append() and attend() run per layer, then
     verify() and commit() once, after which `history` holds the new lengths (on the device, ready for the
-    next plan()). All buffers are made here: a step after plan() allocates nothing and can be captured
-    in a graph; one object serves one stream at a time."""
+    next plan(); a sequence whose commit is refused, which `status` tells, keeps its old one). All buffers
+    are made here: a step after plan() allocates nothing and can be captured in a graph; one object serves
+    one stream at a time."""
 
     def __init__(self, batch: int, tokens: int, num_q_heads: int, num_kv_heads: int, device="cuda",
                  dtype: torch.dtype = torch.bfloat16):
@@ -1215,4 +1221,4 @@ class DraftTree:
     def commit(self, k_cache, v_cache, *, layout: KvLayout, layers: int = 1, **kw) -> None:
         tree_commit(k_cache, v_cache, num_kv_heads=self.num_kv_heads, layout=layout, layers=layers,
                     seq_lens_dev=self.lens, path=self.path, kept=self.kept, seq_lens_out=self.history,
-                    tree_sizes=self.sizes, status=self.status, **kw)
+                    tree_sizes=self.sizes, status=self.status, keep_history=True, **kw)

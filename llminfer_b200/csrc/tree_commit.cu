@@ -28,6 +28,7 @@ struct CommitArgs {
     int32_t elem_bytes;
     int32_t cols;          // 16-byte columns of a row of all heads
     int32_t cols_per_head;
+    int32_t keep_history;  // what a skipped sequence leaves in lens_out: its history, else its length
 };
 
 // grid.x: blocks of kThreads columns, K and V side by side; grid.y: layers; grid.z: sequences.
@@ -56,8 +57,14 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const CommitArgs 
     }
     ok = __syncthreads_and(ok);
     if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) {
-        if (!ok) raise_bad_input(a.cache.status);
-        a.lens_out[b] = ok ? span.base + kept : __ldg(a.cache.seq_lens + b);
+        int32_t len = span.base + kept;
+        if (!ok) {
+            raise_bad_input(a.cache.status);
+            len = __ldg(a.cache.seq_lens + b);
+            const int32_t n = a.cache.tree_sizes != nullptr ? __ldg(a.cache.tree_sizes + b) : a.cache.tokens;
+            if (a.keep_history && n >= 0 && n <= a.cache.tokens && len >= n) len -= n;
+        }
+        a.lens_out[b] = len;
     }
     if (!ok) return;
     const int col = blockIdx.x * kThreads + tid;
@@ -85,11 +92,7 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const CommitArgs 
     }
 }
 
-}  // namespace
-}  // namespace gqa
-
-extern "C" int gqa_tree_commit(const gqa_tree_commit_params* p) {
-    using namespace gqa;
+int commit(const gqa_tree_commit_params* p, bool keep_history) {
     if (p == nullptr) return GQA_ERR_NULL;
     CommitArgs a;
     std::memset(&a, 0, sizeof(a));
@@ -114,6 +117,7 @@ extern "C" int gqa_tree_commit(const gqa_tree_commit_params* p) {
     a.path = p->path;
     a.kept = p->kept;
     a.lens_out = p->seq_lens_out;
+    a.keep_history = keep_history ? 1 : 0;
     a.cols_per_head = kHeadDim * a.elem_bytes / 16;
     a.cols = p->num_kv_heads * a.cols_per_head;
     const dim3 grid((unsigned)((2 * a.cols + kThreads - 1) / kThreads), (unsigned)p->num_layers,
@@ -122,3 +126,14 @@ extern "C" int gqa_tree_commit(const gqa_tree_commit_params* p) {
                                      reinterpret_cast<cudaStream_t>(p->stream), a);
     return e == cudaSuccess ? GQA_OK : GQA_ERR_CUDA;
 }
+
+}  // namespace
+}  // namespace gqa
+
+extern "C" {
+
+int gqa_tree_commit(const gqa_tree_commit_params* p) { return gqa::commit(p, false); }
+
+int gqa_tree_commit_history(const gqa_tree_commit_params* p) { return gqa::commit(p, true); }
+
+}  // extern "C"

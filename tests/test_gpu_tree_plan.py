@@ -1,4 +1,5 @@
-"""Tree drafting on the GPU, what lies between the four calls."""
+"""Tree drafting on the GPU, what lies between the four calls: plans from buffers that the caller goes on to
+use, commits that are refused."""
 import pytest
 import torch
 
@@ -36,3 +37,49 @@ def test_plan_is_done_with_its_inputs_when_it_returns(gqa, kind):
     assert torch.equal(tree.parents.cpu(), PARENTS.int()) and tree.sizes.tolist() == [6, 4]
     assert tree.history.tolist() == [20, 30] and tree.lens.tolist() == [26, 34]
     assert torch.equal(tree.mask.cpu(), mask) and torch.equal(tree.depth.cpu(), depth)
+
+
+@pytest.mark.parametrize("history,path,kept,missing", [
+    (40, [0, 3, 2, -1, -1, -1], 3, False),   # does not ascend
+    (40, [0, 1, 2, 3, 5, 4], 6, False),      # as many as there are, out of order
+    (40, [0, 1, 2, 3, 4, 5], 7, False),      # more than there are
+    (40, [0, 1, 2, 3, 4, 5], -1, False),
+    (40, [0, 2, -1, -1, -1, -1], 2, True),   # the slots have no block
+    (62, [0, 2, -1, -1, -1, -1], 2, False),  # the tree reaches beyond the sequence's blocks
+])
+def test_a_refused_commit_leaves_the_history(gqa, history, path, kept, missing):
+    """Nodes that nobody accepted do not become history: the next plan starts where this one did."""
+    gen = torch.Generator().manual_seed(5)
+    layout = gqa.layout_pool(4, 32, 2)
+    k, v = (torch.randn(4, 2, 32, D, generator=gen).to(BF16).to(DEV) for _ in range(2))
+    k0, v0 = k.clone(), v.clone()
+    tree = gqa.DraftTree(2, 6, 8, 2, DEV)
+    tree.plan(PARENTS, None, torch.tensor([20, history]))
+    tree.path.copy_(ints([[0, 2, 5, -1, -1, -1], path]))
+    tree.kept.copy_(ints([3, kept]))
+    tree.commit(k, v, layout=layout, block_table=ints([[0, 1], [2, -1 if missing else 3]]))
+    assert int(tree.status) == 3
+    assert tree.history.tolist() == [23, history]
+    for c, c0 in ((k, k0), (v, v0)):
+        for i, node in enumerate([0, 2, 5]):
+            c0[0, :, 20 + i] = c0[0, :, 20 + node].clone()
+        assert torch.equal(c, c0)
+    tree.plan(PARENTS, torch.tensor([6, 5]))
+    assert tree.lens.tolist() == [29, history + 5]
+
+
+def test_the_history_of_an_accepted_commit(gqa):
+    """All nodes, some, the root, none of an empty tree: the same lengths from both forms of the call."""
+    layout = gqa.layout_pool(4, 32, 2)
+    k, v = (torch.zeros(4, 2, 32, D, dtype=BF16, device=DEV) for _ in range(2))
+    table, parents = ints([[0], [1], [2], [3]]), PARENTS[:1].expand(4, 6)
+    tree = gqa.DraftTree(4, 6, 8, 2, DEV)
+    tree.plan(parents, torch.tensor([6, 6, 3, 0]), torch.tensor([26, 5, 0, 7]))
+    tree.path.copy_(ints([[0, 1, 2, 3, 4, 5], [0, 1, 3, -1, -1, -1], [0, -1, -1, -1, -1, -1], [-1] * 6]))
+    tree.kept.copy_(ints([6, 3, 1, 0]))
+    plain = ints([0] * 4)
+    gqa.tree_commit(k, v, num_kv_heads=2, layout=layout, seq_lens_dev=tree.lens, path=tree.path, kept=tree.kept, seq_lens_out=plain,
+                    tree_sizes=tree.sizes, block_table=table)
+    tree.commit(k, v, layout=layout, block_table=table)
+    assert int(tree.status) == 0
+    assert tree.history.tolist() == plain.tolist() == [32, 8, 1, 7]

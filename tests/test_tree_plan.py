@@ -1,6 +1,10 @@
-"""DraftTree.plan on the host: what it takes and what it leaves in the buffers."""
+"""Tree drafting without a GPU: what DraftTree.plan takes and leaves in the buffers, refusals."""
+import ctypes as C
+
 import pytest
 import torch
+
+from test_tree_host import COMMON, _fill
 
 
 @pytest.fixture(scope="module")
@@ -40,3 +44,11 @@ def test_plan_fills_the_buffers(tree, kind):
     assert torch.equal(tree.parents, PARENTS.int())
     tree.plan(PARENTS)  # from the lengths that are there
     assert tree.lens.tolist() == [9, 10] and tree.sizes.tolist() == [4, 4]
+
+
+@pytest.mark.parametrize("kw,code", COMMON + [(dict(path=None), -1), (dict(num_layers=0), -3), (dict(seq_lens_out=0x2000, kept=0x2000), -8)])
+def test_tree_commit_history_refuses_what_tree_commit_refuses(gqa, kw, code):
+    from llminfer_b200 import binding as B
+    p = _fill(B._TreeCommitParams(), gqa, **{**dict(num_layers=1, seq_lens_out=0x3000), **kw})
+    assert gqa.lib().gqa_tree_commit_history(C.byref(p)) == code
+    assert gqa.lib().gqa_tree_commit_history(None) == -1
