@@ -819,8 +819,8 @@ int gqa_tree_verify(const gqa_tree_verify_params* p);
  * Keeps the accepted path: in every layer, the K and V rows of slot seq_len - n_b + path[b, i] move to
  * slot seq_len - n_b + i for i < kept[b], in place, and seq_lens_out[b] = seq_len - n_b + kept[b].
  * path must ascend (path[i] > path[i - 1], path[i] < n_b), as gqa_tree_verify leaves it; a sequence whose
- * path does not, or whose kept is outside 0 .. n_b, is skipped with its length unchanged
- * (GQA_STATUS_BAD_INPUT): seq_lens_out[b] = seq_len, which still counts the nodes. A loop that takes
+ * path does not, whose kept is outside 0 .. n_b, or of whose kept rows one has no block, is skipped with its
+ * length unchanged (GQA_STATUS_BAD_INPUT): seq_lens_out[b] = seq_len, which still counts the nodes. A loop that takes
  * seq_lens_out as the next step's history calls gqa_tree_commit_history, where a skipped sequence keeps
  * its history instead. Slots behind the kept rows are left as they are.
  *   dtype            GQA_DTYPE_BF16 or GQA_DTYPE_F32 (rows are moved bit for bit).

@@ -49,9 +49,8 @@ __global__ void __launch_bounds__(kThreads) tree_commit_kernel(const CommitArgs 
         const int32_t from = s_path[tid];
         ok = from < span.n && from > (tid > 0 ? s_path[tid - 1] : -1);
         int64_t src = 0, dst = 0;
-        if (ok && from != tid) {
-            ok = tree_row(a.cache, b, span.base + from, &src) && tree_row(a.cache, b, span.base + tid, &dst);
-        }
+        // Rows that stay are looked up too: without a block nothing can have been written there.
+        if (ok) ok = tree_row(a.cache, b, span.base + from, &src) && tree_row(a.cache, b, span.base + tid, &dst);
         s_src[tid] = from != tid ? src * a.elem_bytes : -1;
         s_dst[tid] = dst * a.elem_bytes;
     }

@@ -83,3 +83,21 @@ def test_the_history_of_an_accepted_commit(gqa):
     tree.commit(k, v, layout=layout, block_table=table)
     assert int(tree.status) == 0
     assert tree.history.tolist() == plain.tolist() == [32, 8, 1, 7]
+
+
+@pytest.mark.parametrize("path,kept", [([0, 1, -1, -1, -1, -1], 2), ([0, 1, 3, -1, -1, -1], 3)])
+@pytest.mark.parametrize("missing", [-1, 4])
+def test_commit_refuses_kept_rows_without_a_block(gqa, path, kept, missing):
+    """Rows that stay where they are must have a place too: no other call could have written them."""
+    layout = gqa.layout_pool(4, 32, 2)
+    k, v = (torch.ones(4, 2, 32, D, dtype=BF16, device=DEV) for _ in range(2))
+    new, status = ints([0]), ints([0])
+    kw = dict(num_kv_heads=2, layout=layout, path=ints([path]), kept=ints([kept]), seq_lens_out=new, block_table=ints([[2, missing]]), status=status)
+    gqa.tree_commit(k, v, seq_lens_dev=ints([37]), **kw)   # nodes in slots 31 .. 36
+    assert int(status) == 3 and int(new) == 37 and (k == 1).all() and (v == 1).all()
+    status.zero_()
+    gqa.tree_commit(k, v, seq_lens_dev=ints([37]), keep_history=True, **kw)
+    assert int(status) == 3 and int(new) == 31
+    status.zero_()
+    gqa.tree_commit(k, v, seq_lens_dev=ints([32]), **kw)   # 26 .. 31
+    assert int(status) == 0 and int(new) == 26 + kept
