@@ -109,7 +109,7 @@ int commit(const gqa_tree_commit_params* p, bool keep_history) {
         return GQA_ERR_UNSUPPORTED;
     }
     a.elem_bytes = p->dtype == GQA_DTYPE_F32 ? 4 : 2;
-    a.layer_bytes = p->layer_stride * a.elem_bytes;
+    a.layer_bytes = p->num_layers > 1 ? p->layer_stride * a.elem_bytes : 0;
     if (a.layer_bytes % 16 != 0) return GQA_ERR_ALIGN;
     a.k_cache = p->k_cache;
     a.v_cache = p->v_cache;

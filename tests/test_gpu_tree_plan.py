@@ -101,3 +101,18 @@ def test_commit_refuses_kept_rows_without_a_block(gqa, path, kept, missing):
     status.zero_()
     gqa.tree_commit(k, v, seq_lens_dev=ints([32]), **kw)   # 26 .. 31
     assert int(status) == 0 and int(new) == 26 + kept
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_commit_of_one_layer_in_a_buffer_of_odd_size(gqa, dtype):
+    """With one layer there is no distance between layers to be aligned."""
+    gen = torch.Generator().manual_seed(6)
+    layout = gqa.layout_reference(1, 32, 2)
+    k, v = (torch.randn(32 * 2 * D + 3, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    want = [c.clone() for c in (k, v)]
+    for c in want:
+        c[: 32 * 2 * D].view(32, 2, D)[17] = c[: 32 * 2 * D].view(32, 2, D)[18].clone()
+    new = ints([0])
+    gqa.tree_commit(k, v, num_kv_heads=2, layout=layout, seq_lens_dev=ints([20]), path=ints([[0, 2, -1, -1]]), kept=ints([2]),
+                    seq_lens_out=new)
+    assert int(new) == 18 and torch.equal(k, want[0]) and torch.equal(v, want[1])
