@@ -734,7 +734,8 @@ int gqa_rope_append(const gqa_rope_params* p);
  *   q, out         [batch, tokens, num_q_heads, 128], q_token_stride elements between tokens of q (0:
  *                  packed; sequences follow at tokens * stride), out packed and not on top of q.
  *                  num_q_heads / num_kv_heads <= 8.
- *   layout, block_table_dev, blocks_per_seq, fixed_block   as in gqa_decode_params; batch <= 1024.
+ *   layout, block_table_dev, blocks_per_seq, fixed_block   as in gqa_decode_params; batch <= 1024, at most
+ *                  2^31 - 129 positions per sequence (GQA_ERR_SHAPE).
  *   workspace      gqa_tree_workspace_bytes() bytes, 16-byte aligned, no initialisation; calls that
  *                  may overlap (streams, concurrent graph launches) need one each.
  */

@@ -5,6 +5,8 @@
 
 namespace gqa {
 
+constexpr int kTreeTileKeys = 128;  // keys of a place in the cut of tree_cut.cuh
+
 struct TreeArgs {
     TreeCache cache;
     const void* q;

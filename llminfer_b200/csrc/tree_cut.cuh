@@ -10,7 +10,7 @@
 namespace gqa {
 namespace {
 
-constexpr int kTile = 128;    // keys per place
+constexpr int kTile = kTreeTileKeys;
 constexpr int kUnitPad = 1;   // places a unit counts on top of its tiles
 constexpr int kRecordCols = kHeadDim + 2;
 constexpr int kLongList = 30;  // records of a unit that a merge shares among its threads

@@ -47,6 +47,8 @@ int gqa_tree_decode(const gqa_tree_decode_params* p) {
     if (!shape_ok(p->dtype, p->batch, p->tokens, p->num_q_heads, p->num_kv_heads)) {
         return GQA_ERR_UNSUPPORTED;
     }
+    // Keys are counted up to the end of a tile in 32 bits.
+    if (a.cache.capacity > INT32_MAX - kTreeTileKeys) return GQA_ERR_SHAPE;
     if (p->q == nullptr || p->out == nullptr || p->workspace == nullptr) return GQA_ERR_NULL;
     const int64_t eb = p->dtype == GQA_DTYPE_F32 ? 4 : 2;
     const int64_t q_row = (int64_t)p->num_q_heads * kHeadDim;

@@ -52,3 +52,13 @@ def test_tree_commit_history_refuses_what_tree_commit_refuses(gqa, kw, code):
     p = _fill(B._TreeCommitParams(), gqa, **{**dict(num_layers=1, seq_lens_out=0x3000), **kw})
     assert gqa.lib().gqa_tree_commit_history(C.byref(p)) == code
     assert gqa.lib().gqa_tree_commit_history(None) == -1
+
+
+@pytest.mark.parametrize("dtype", [1, 2])
+@pytest.mark.parametrize("block,blocks,code", [(64, (1 << 25) - 1, -3), (32, (1 << 26) - 1, -3), (64, 1 << 25, -3)])
+def test_tree_decode_refuses_positions_that_tiles_of_keys_would_carry_past_32_bits(gqa, dtype, block, blocks, code):
+    """Capacities of 2^31 - 64, 2^31 - 32 and 2^31: the end of the last tile of 128 keys is no 32-bit number."""
+    from llminfer_b200 import binding as B
+    p = _fill(B._TreeDecodeParams(), gqa, dtype=dtype, workspace_bytes=1 << 40, out=0x2000, blocks_per_seq=blocks,
+              layout=gqa.layout_pool(8, block, 2).c())
+    assert gqa.lib().gqa_tree_decode(C.byref(p)) == code
