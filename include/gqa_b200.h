@@ -732,7 +732,8 @@ int gqa_rope_append(const gqa_rope_params* p);
  * infinities and NaN included.
  *   dtype          GQA_DTYPE_BF16 or GQA_DTYPE_F32 (q, out and caches).
  *   q, out         [batch, tokens, num_q_heads, 128], q_token_stride elements between tokens of q (0:
- *                  packed; sequences follow at tokens * stride), out packed and not on top of q.
+ *                  packed; sequences follow at tokens * stride), out packed and outside the rows of q
+ *                  (GQA_ERR_UNSUPPORTED).
  *                  num_q_heads / num_kv_heads <= 8.
  *   layout, block_table_dev, blocks_per_seq, fixed_block   as in gqa_decode_params; batch <= 1024, at most
  *                  2^31 - 129 positions per sequence (GQA_ERR_SHAPE).

@@ -84,6 +84,24 @@ struct TreeCacheDesc {
 };
 int tree_cache_args(const TreeCacheDesc& d, TreeCache* out);
 
+// Whether n rows of `bytes` bytes, a_step apart from a on, share a byte with those b_step apart from b on (steps of
+// `bytes` at least; host). Two comparisons unless the spans meet.
+inline bool rows_overlap(const void* a, int64_t a_step, const void* b, int64_t b_step, int64_t n, int64_t bytes) {
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+    if (a0 + (n - 1) * a_step + bytes <= b0 || b0 + (n - 1) * b_step + bytes <= a0) return false;
+    for (int64_t i = 0, j = 0; i < n && j < n;) {
+        const uintptr_t row_a = a0 + i * a_step, row_b = b0 + j * b_step;
+        if (row_a + bytes <= row_b) {
+            ++i;
+        } else if (row_b + bytes <= row_a) {
+            ++j;
+        } else {
+            return true;
+        }
+    }
+    return false;
+}
+
 // Tensor maps of the tree attention kernel, encoded anew for every call. The cache as (channel,
 // token / head by ascending stride, block) with boxes of box_keys rows x 64 channels of one head; the
 // queries as (channel, head, row of tokens) with boxes of 64 channels x group heads x box_tokens.

@@ -57,7 +57,10 @@ int gqa_tree_decode(const gqa_tree_decode_params* p) {
     if (!aligned16(p->q) || !aligned16(p->out) || !aligned16(p->workspace) || a.q_stride * eb % 16) {
         return GQA_ERR_ALIGN;
     }
-    if (p->out == p->q) return GQA_ERR_UNSUPPORTED;  // rows of one head are written while others are still to be read
+    // Rows of one head are written while others are still to be read.
+    if (rows_overlap(p->q, a.q_stride * eb, p->out, q_row * eb, (int64_t)p->batch * p->tokens, q_row * eb)) {
+        return GQA_ERR_UNSUPPORTED;
+    }
     int32_t sms = 0;
     if (current_sm_count(&sms) != GQA_OK) return GQA_ERR_CUDA;
     if (p->workspace_bytes < gqa_tree_workspace_bytes(p->dtype, p->batch, p->tokens, p->num_q_heads,

@@ -62,3 +62,13 @@ def test_tree_decode_refuses_positions_that_tiles_of_keys_would_carry_past_32_bi
     p = _fill(B._TreeDecodeParams(), gqa, dtype=dtype, workspace_bytes=1 << 40, out=0x2000, blocks_per_seq=blocks,
               layout=gqa.layout_pool(8, block, 2).c())
     assert gqa.lib().gqa_tree_decode(C.byref(p)) == code
+
+
+ROW = 4 * 128 * 2  # bytes of a token's queries below
+
+
+@pytest.mark.parametrize("offset,stride", [(16, 0), (-16, 0), (7 * ROW, 0), (-7 * ROW, 0), (-8 * ROW + 16, 0), (ROW, 1024), (ROW - 16, 1024), (14 * ROW, 1024)])
+def test_tree_decode_refuses_output_that_reaches_into_the_queries(gqa, offset, stride):
+    from llminfer_b200 import binding as B
+    p = _fill(B._TreeDecodeParams(), gqa, workspace_bytes=1 << 40, q=0x100000, out=0x100000 + offset, q_token_stride=stride)
+    assert gqa.lib().gqa_tree_decode(C.byref(p)) == -8
