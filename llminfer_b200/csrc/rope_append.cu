@@ -310,6 +310,10 @@ extern "C" int gqa_rope_append(const gqa_rope_params* p) {
     }
     // In place means row on row: with another stride a warp would overwrite rows not yet read.
     if (p->q == p->q_out && a.q_stride != a.q_out_stride) return GQA_ERR_SHAPE;
+    if (p->q != p->q_out && rows_overlap(p->q, a.q_stride * eb, p->q_out, a.q_out_stride * eb,
+                                         (int64_t)p->batch * p->tokens, q_row * eb)) {
+        return GQA_ERR_UNSUPPORTED;
+    }
     a.q = p->q;
     a.q_out = p->q_out;
     a.k_new = p->k_new;

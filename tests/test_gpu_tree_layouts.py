@@ -110,3 +110,21 @@ def test_fp32_queries_inside_packed_rows(gqa):
         outs.append(torch.zeros(2, tokens, hq, D, device=DEV))
         gqa.tree_decode(q, k, v, outs[-1], num_kv_heads=hkv, layout=layout, seq_lens_dev=ints(lens), block_table=table, workspace=ws)
     assert torch.equal(outs[0], outs[1]) and outs[0].abs().sum() > 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_between_rows(gqa, dtype):
+    """Queries and outputs that lie in one buffer without sharing an element: the same bits as apart."""
+    gen = torch.Generator().manual_seed(8)
+    hq, hkv, tokens = 4, 2, 6
+    rows = torch.randn(2, tokens, 3 * hq, D, generator=gen).to(dtype).to(DEV)
+    q, q_out = rows[:, :, :hq], rows[:, :, 2 * hq:]
+    before = rows.clone()
+    kn, vn = (torch.randn(2, tokens, hkv, D, generator=gen).to(dtype).to(DEV) for _ in range(2))
+    k, v = (torch.zeros(4, hkv, 32, D, dtype=dtype, device=DEV) for _ in range(2))
+    freq, _ = gqa.rope_frequencies(128)
+    kw = dict(layout=gqa.layout_pool(4, 32, hkv), seq_lens_dev=ints([40, 20]), freq=freq.to(DEV), block_table=ints([[0, 1], [2, 3]]))
+    apart = torch.zeros(2, tokens, hq, D, dtype=dtype, device=DEV)
+    gqa.rope_append(q.contiguous(), kn, vn, k, v, q_out=apart, **kw)
+    gqa.rope_append(q, kn, vn, k, v, q_out=q_out, **kw)
+    assert torch.equal(q_out, apart) and torch.equal(rows[:, :, : 2 * hq], before[:, :, : 2 * hq]) and apart.abs().sum() > 0

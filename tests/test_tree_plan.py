@@ -72,3 +72,13 @@ def test_tree_decode_refuses_output_that_reaches_into_the_queries(gqa, offset, s
     from llminfer_b200 import binding as B
     p = _fill(B._TreeDecodeParams(), gqa, workspace_bytes=1 << 40, q=0x100000, out=0x100000 + offset, q_token_stride=stride)
     assert gqa.lib().gqa_tree_decode(C.byref(p)) == -8
+
+
+@pytest.mark.parametrize("offset,stride,out_stride", [(16, 0, 0), (-16, 0, 0), (ROW, 0, 0), (-7 * ROW, 0, 0), (ROW - 16, 1280, 1280), (6 * ROW, 1280, 512),
+                                                      (-2 * ROW, 512, 1280)])
+def test_rope_append_refuses_rows_that_reach_into_one_another(gqa, offset, stride, out_stride):
+    """In place is row on row; any other way to share memory overwrites rows that are still to be read."""
+    from llminfer_b200 import binding as B
+    p = _fill(B._RopeParams(), gqa, rotary_dim=128, eps=1e-6, attn_factor=1.0, q=0x100000, q_out=0x100000 + offset, q_token_stride=stride,
+              q_out_token_stride=out_stride)
+    assert gqa.lib().gqa_rope_append(C.byref(p)) == -8
