@@ -830,8 +830,8 @@ int gqa_tree_verify(const gqa_tree_verify_params* p);
  *   num_layers, layer_stride   the caches of layer l start l * layer_stride elements behind k_cache /
  *                    v_cache; layout and block table are the same for all layers. layer_stride means
  *                    nothing where there is one layer.
- *   seq_lens_out     must not be seq_lens_dev, tree_sizes_dev, path or kept: other blocks of the launch still read
- *                    those (GQA_ERR_UNSUPPORTED).
+ *   seq_lens_out     shares no element with seq_lens_dev, tree_sizes_dev, path or kept: other blocks of the launch
+ *                    still read those (GQA_ERR_UNSUPPORTED).
  */
 typedef struct gqa_tree_commit_params {
     int32_t dtype;

@@ -104,10 +104,12 @@ int commit(const gqa_tree_commit_params* p, bool keep_history) {
     if (p->num_layers <= 0 || p->num_layers > 65535 || p->batch > 65535) return GQA_ERR_SHAPE;
     if (p->num_layers > 1 && p->layer_stride <= 0) return GQA_ERR_SHAPE;
     // One block of a sequence writes its length while the others still read these.
-    if (p->seq_lens_out == p->seq_lens_dev || p->seq_lens_out == p->kept || p->seq_lens_out == p->tree_sizes_dev ||
-        p->seq_lens_out == p->path) {
-        return GQA_ERR_UNSUPPORTED;
+    const int64_t lens_bytes = (int64_t)p->batch * sizeof(int32_t);
+    for (const int32_t* in : {p->seq_lens_dev, p->kept, p->tree_sizes_dev}) {
+        if (in != nullptr && rows_overlap(p->seq_lens_out, 0, in, 0, 1, lens_bytes)) return GQA_ERR_UNSUPPORTED;
     }
+    const uintptr_t out = reinterpret_cast<uintptr_t>(p->seq_lens_out), path = reinterpret_cast<uintptr_t>(p->path);
+    if (out + lens_bytes > path && out < path + lens_bytes * p->tokens) return GQA_ERR_UNSUPPORTED;
     a.elem_bytes = p->dtype == GQA_DTYPE_F32 ? 4 : 2;
     a.layer_bytes = p->num_layers > 1 ? p->layer_stride * a.elem_bytes : 0;
     if (a.layer_bytes % 16 != 0) return GQA_ERR_ALIGN;

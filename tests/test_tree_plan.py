@@ -82,3 +82,13 @@ def test_rope_append_refuses_rows_that_reach_into_one_another(gqa, offset, strid
     p = _fill(B._RopeParams(), gqa, rotary_dim=128, eps=1e-6, attn_factor=1.0, q=0x100000, q_out=0x100000 + offset, q_token_stride=stride,
               q_out_token_stride=out_stride)
     assert gqa.lib().gqa_rope_append(C.byref(p)) == -8
+
+
+@pytest.mark.parametrize("name,size", [("seq_lens_dev", 2), ("tree_sizes_dev", 2), ("kept", 2), ("path", 8)])
+def test_tree_commit_refuses_lengths_that_reach_into_its_inputs(gqa, name, size):
+    """Two sequences of four nodes: outputs that begin below an input's end or end above its beginning."""
+    from llminfer_b200 import binding as B
+    for at in (-1, 1, size - 1):
+        p = _fill(B._TreeCommitParams(), gqa, num_layers=1, seq_lens_out=0x3000 + 4 * at, **{name: 0x3000})
+        for call in (gqa.lib().gqa_tree_commit, gqa.lib().gqa_tree_commit_history):
+            assert call(C.byref(p)) == -8, at
