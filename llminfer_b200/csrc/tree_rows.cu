@@ -41,8 +41,6 @@ struct Shape {
     static constexpr size_t kBytes = (size_t)(kQ + kStages * kStage + kWeights) * sizeof(float);
 };
 
-size_t table_room(int batch) { return (3 * (size_t)batch + 1) * sizeof(int32_t); }
-
 // 16 bytes to shared memory, zeros when `some` is false (the source is not read then).
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool some) {
     const uint32_t bytes = some ? 16u : 0u;
@@ -299,7 +297,7 @@ int tile_rows_of(int32_t tokens, int32_t group) {
 
 template <int RT>
 int launch(const TreeArgs& a, cudaStream_t stream) {
-    const size_t smem = Shape<RT>::kBytes + table_room(a.batch);
+    const size_t smem = Shape<RT>::kBytes + table_bytes(a.batch);
     auto kernel = tree_rows_kernel<RT>;
     {
         static std::mutex mu;
