@@ -632,7 +632,9 @@ int gqa_qkv_gemv(const gqa_qkv_params* p);
  * in slot seq_len - n_b + t. n_b may differ from sequence to sequence and may be 0 (nothing to do).
  * Rows t >= n_b of per-node outputs are left as they were. A sequence whose length or size is out of
  * range (n_b < 0, n_b > tokens, seq_len < n_b, seq_len beyond what its blocks hold) is skipped and
- * *status_dev (optional) set to GQA_STATUS_BAD_INPUT. At most GQA_TREE_MAX_TOKENS nodes.
+ * *status_dev (optional) set to GQA_STATUS_BAD_INPUT. So it is where a position's block table entry names no
+ * block: rotary append leaves such rows out, attention takes them for rows of zeros, commit skips the sequence.
+ * At most GQA_TREE_MAX_TOKENS nodes.
  * The four wait for earlier work of the stream before they read anything, and may be captured in graphs.
  * Behind them gqa_decode_params.early_prefetch is not to be set until the stream has been synchronised (or
  * a launch of another library waited): they write lengths and rows of more than the newest position.
@@ -659,7 +661,12 @@ int gqa_tree_masks(const int32_t* parents, const int32_t* sizes, int32_t batch, 
 #define GQA_ROPE_SCALE_NTK 2    /* base * factor^(r / (r - 2)), r = rotary_dim > 2 */
 #define GQA_ROPE_SCALE_YARN 3   /* YaRN: pairs that turn less than beta_slow times over original_len
                                    positions divided by `factor`, those above beta_fast kept, the rest
-                                   interpolated linearly in the number of turns */
+                                   interpolated linearly in the number of turns, the ramp of the method's
+                                   paper. Programs that serve published checkpoints often take a ramp that is
+                                   linear in the pair's index between the two ends instead, which gives
+                                   other angles (up to 1.7 times for a pair at base 1e6, factor 4, 32768
+                                   positions): where a checkpoint was trained with such frequencies, pass
+                                   those as freq_dev. */
 
 /*
  * Host only: freq[rotary_dim / 2] in radians per position, FP64, and the factor sine and cosine are

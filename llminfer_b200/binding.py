@@ -994,7 +994,9 @@ def tree_masks(parents: torch.Tensor, sizes: Optional[torch.Tensor] = None):
 def rope_frequencies(rotary_dim: int = 128, base: float = 1e6, scaling: str = "none",
                      factor: float = 1.0, original_len: int = 0, beta_fast: float = 32.0,
                      beta_slow: float = 1.0):
-    """Radians per position of each rotated pair (FP64, on the host) and the attention factor."""
+    """Radians per position of each rotated pair (FP64, on the host) and the attention factor. "yarn"
+    interpolates linearly in a pair's turns over original_len positions, not in its index as programs that serve
+    published checkpoints often do: rope_append takes any frequencies."""
     freq = torch.zeros(max(rotary_dim // 2, 1), dtype=torch.float64)
     attn = C.c_float()
     _check(lib().gqa_rope_frequencies(rotary_dim, base, ROPE_SCALINGS[scaling], factor, original_len,

@@ -128,3 +128,18 @@ def test_rows_between_rows(gqa, dtype):
     gqa.rope_append(q.contiguous(), kn, vn, k, v, q_out=apart, **kw)
     gqa.rope_append(q, kn, vn, k, v, q_out=q_out, **kw)
     assert torch.equal(q_out, apart) and torch.equal(rows[:, :, : 2 * hq], before[:, :, : 2 * hq]) and apart.abs().sum() > 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("entry", [-1, 4, 1 << 30])
+def test_positions_without_a_block_are_rows_of_zeros(gqa, dtype, entry):
+    gen = torch.Generator().manual_seed(9)
+    hq, hkv, tokens, length = 8, 2, 5, 110
+    k, v = (torch.randn(4, hkv, 32, D, generator=gen).to(dtype) for _ in range(2))
+    q, status = torch.randn(1, tokens, hq, D, generator=gen).to(dtype), ints([0])
+    out = torch.zeros(1, tokens, hq, D, dtype=dtype, device=DEV)
+    gqa.tree_decode(q.to(DEV), k.to(DEV), v.to(DEV), out, num_kv_heads=hkv, layout=gqa.layout_pool(4, 32, hkv), seq_lens_dev=ints([length]),
+                    block_table=ints([[3, entry, 0, 1]]), workspace=gqa.tree_workspace(1, tokens, hq, hkv, DEV, dtype), status=status)
+    assert int(status) == 3
+    rows = lambda c: torch.cat([c[3], torch.zeros_like(c[0]), c[0], c[1]], 1).transpose(0, 1)[:length]
+    check(out, q, [rows(k)], [rows(v)], [length], [tokens], [np.tril(np.ones((tokens, tokens), dtype=bool))], dtype)

@@ -1,6 +1,8 @@
 """Tree drafting without a GPU: what DraftTree.plan takes and leaves in the buffers, refusals."""
 import ctypes as C
+import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -92,3 +94,17 @@ def test_tree_commit_refuses_lengths_that_reach_into_its_inputs(gqa, name, size)
         p = _fill(B._TreeCommitParams(), gqa, num_layers=1, seq_lens_out=0x3000 + 4 * at, **{name: 0x3000})
         for call in (gqa.lib().gqa_tree_commit, gqa.lib().gqa_tree_commit_history):
             assert call(C.byref(p)) == -8, at
+
+
+@pytest.mark.parametrize("rotary,base,factor,original,fast,slow", [
+    (128, 1e6, 4.0, 32768, 32.0, 1.0), (128, 1e6, 40.0, 4096, 32.0, 1.0), (64, 1e4, 2.0, 2048, 16.0, 2.0), (8, 1e4, 8.0, 131072, 32.0, 1.0)])
+def test_yarn_interpolates_linearly_in_turns(gqa, rotary, base, factor, original, fast, slow):
+    """Every pair, those between the ramp's ends among them: a pair that turns r times over the trained context keeps
+    (r - slow) / (fast - slow) of its frequency, cut to 0 .. 1, and divides the rest by the factor. Both sides take some ten
+    FP64 roundings, of numbers at most 4 times the result: below 1e-14."""
+    f, a = gqa.rope_frequencies(rotary, base=base, scaling="yarn", factor=factor, original_len=original, beta_fast=fast, beta_slow=slow)
+    plain = base ** (-2.0 * np.arange(rotary // 2) / rotary)
+    keep = np.clip((original * plain / (2 * math.pi) - slow) / (fast - slow), 0.0, 1.0)
+    assert rotary < 64 or ((keep > 0) & (keep < 1)).sum() >= 4
+    np.testing.assert_allclose(f.numpy(), plain * (keep + (1.0 - keep) / factor), rtol=1e-14)
+    assert a == pytest.approx(0.1 * math.log(factor) + 1.0, rel=2.0 ** -24)
