@@ -248,6 +248,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
+        if (ok) {
+            // The last releases of the slots arrive by themselves, when the products that read them are complete; nothing else
+            // waits for them, and the block's barriers must not be gone before.
+            for (uint32_t f = fills > (uint32_t)kRing ? fills - kRing : 0; f < fills && ok; ++f) {
+                ok = wait_warp(smem_u32(&s_kv_empty[f % kRing]), (f / kRing) & 1u, dead);
+            }
+            for (uint32_t f = q_fills > q_slots ? q_fills - q_slots : 0; f < q_fills && ok; ++f) {
+                ok = wait_warp(smem_u32(&s_q_empty[f % q_slots]), (f / q_slots) & 1u, dead);
+            }
+        }
         if (!ok) {
             // Copies in flight land before the block ends (again with a limit).
             if (lane == 0) {

@@ -143,3 +143,33 @@ def test_positions_without_a_block_are_rows_of_zeros(gqa, dtype, entry):
     assert int(status) == 3
     rows = lambda c: torch.cat([c[3], torch.zeros_like(c[0]), c[0], c[1]], 1).transpose(0, 1)[:length]
     check(out, q, [rows(k)], [rows(v)], [length], [tokens], [np.tril(np.ones((tokens, tokens), dtype=bool))], dtype)
+
+
+@pytest.mark.parametrize("tokens", [8, 40])
+def test_launches_back_to_back(gqa, tokens):
+    """Blocks follow one another on an SM without a pause: each leaves only when all that was to arrive in its memory has."""
+    gen = torch.Generator().manual_seed(tokens)
+    hq, hkv, batch = 32, 8, 3
+    k, v = (torch.randn(batch, 700, hkv, D, generator=gen).to(BF16).to(DEV) for _ in range(2))
+    q = torch.randn(batch, tokens, hq, D, generator=gen).to(BF16).to(DEV)
+    layout, table, ws = gqa.layout_reference(batch, 700, hkv), ints([[0], [1], [2]]), gqa.tree_workspace(batch, tokens, hq, hkv, DEV)
+    lens = [ints([tokens, 129, 700]), ints([128, tokens + 1, 300]), ints([650, 513, 40])]
+
+    def call(out, n):
+        gqa.tree_decode(q, k, v, out, num_kv_heads=hkv, layout=layout, seq_lens_dev=lens[n], block_table=table, workspace=ws)
+
+    want = [torch.zeros_like(q) for _ in lens]
+    for i, w in enumerate(want):
+        call(w, i)
+        torch.cuda.synchronize()
+    got = [torch.zeros_like(q) for _ in range(90)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i, g in enumerate(got):
+            call(g, i % 3)
+    for _ in range(3):
+        for g in got:
+            g.zero_()
+        graph.replay()
+        for i, g in enumerate(got):
+            assert torch.equal(g, want[i % 3]), i
