@@ -637,7 +637,8 @@ int gqa_qkv_gemv(const gqa_qkv_params* p);
  * At most GQA_TREE_MAX_TOKENS nodes.
  * The four wait for earlier work of the stream before they read anything, and may be captured in graphs.
  * Behind them gqa_decode_params.early_prefetch is not to be set until the stream has been synchronised (or
- * a launch of another library waited): they write lengths and rows of more than the newest position.
+ * a launch of another library waited): they write lengths and rows of more than the newest position. The
+ * C++ shim's attention sets it by itself, so a program that uses both synchronises the stream between them.
  */
 #define GQA_TREE_MAX_TOKENS 128
 

@@ -15,8 +15,8 @@
 // a warp asks for all its heads before it looks at either.
 //
 // Measured: 64 sequences of up to 64 nodes (48 on average), 64 / 8 heads, BF16, norm: 32 us, 3.9 TB/s of rows read and
-// written (0.60 of a copy); bound by the life of a block (load, angles, norm, store) at the 25 warps per SM that 80
-// registers leave. Fewer heads per warp: 34 us with 8, 36 with 2; 8 nodes of 32 / 8 heads: 2.5 us, a launch.
+// written (0.59 of a copy); bound by the life of a block (load, angles, norm, store) at the 25 warps per SM that 80
+// registers leave. Fewer heads per warp: 34 us with 8, 36 with 2; 8 nodes of 32 / 8 heads: 2.5 - 2.9 us, a launch.
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -28,7 +28,7 @@ namespace gqa {
 namespace {
 
 constexpr int kMaxWarps = 8;  // of a block
-// Pairs of heads of a warp, all in flight: 64 bytes a lane.
+// Pairs of heads of a warp, all in flight: 128 bytes a lane.
 template <typename T> constexpr int kPairs = 32 / (int)sizeof(T) / 2;
 
 struct RopeArgs {

@@ -4,9 +4,13 @@
 // a tile of keys is 128 positions of the cache. S = Q K^T and O += P V run as 128 x 128 x 128 products with
 // FP32 accumulators in tensor memory, P = 2^(c (S - m)) with the running maximum m and sum l in FP32
 // registers, one thread per row. P is rounded to BF16 for the second product (V is BF16 and both operands
-// have one type); the sum takes the unrounded weights. m is only moved when a tile's maximum exceeds it by 2^8:
-// the weights then stay below 2^8, their relative rounding is the same, and O (in tensor memory) is
-// rescaled a few times per sequence instead of once per tile.
+// have one type); the sum takes the unrounded weights, which saves two instructions per pair in a loop of about
+// five. m is only moved when a tile's maximum exceeds it by 2^8 (a published idea): the weights then stay
+// below 2^8, and O (in tensor memory) is rescaled a few times per sequence instead of once per tile. A weight is off by at most
+// half a step (2^-8 of it at its binade's start), so the output is off by that part of the weighted mean of |v| before its own
+// rounding. Where one key has nearly all the weight that is a common factor, up to 2^-8 away from 1 unless the
+// weight is a power of two: gqa_decode, which sums the rounded weights, returns such a value row unchanged.
+// Relative to FP64, all outputs of a measured case together: 0.0022 - 0.0024 (FP32 weights: 0.0017, the output's rounding).
 //
 // A CTA has two streams of softmax, a warpgroup each. With one query tile (rows <= 128) the streams
 // take the key tiles in turn, each with its own O, m and l, merged at the end; with two query tiles they
@@ -25,9 +29,11 @@
 // rows past the end are zeroed in shared memory (0 * NaN). A node's V row that holds an infinity or
 // NaN is zeroed too, and added by hand to the rows that see it, in the epilogue.
 //
-// Measured (32 / 8 heads unless stated): 16 sequences of 256 - 8192 keys, 16 nodes: 66 us, 4.5 TB/s; 64 nodes of 64 / 8
-// heads over 32768 keys: 86 us, 800 TFLOP/s, bound by the chain of a stream's products and weights; 8 nodes over 1024 keys: 11 us with the
-// merge; 4 x 131072 keys, 64 / 8 heads, 8 nodes: 313 - 335 us in a short burst, 381 us at the clock of a long one.
+// Measured in a graph, the merge included (32 / 8 heads unless stated): 16 sequences of 256 - 8192 keys, 16 nodes: 66 us, 4.2 TB/s of
+// keys and values; 64 nodes of 64 / 8 heads over 32768 keys: 86 us, 800 TFLOP/s (call after call from a host program: 101 us, 680); tensor
+// pipe, exponentials and issue each a quarter busy at 8192 keys: two softmax warps per scheduler wait for tensor memory and
+// barriers; 8 nodes over 1024 keys: 11.4 us; 4 x 131072 keys, 64 / 8 heads, 8 nodes: 313 - 335 us in a short burst, 390 us at the
+// clock of a long one.
 #include <cuda_bf16.h>
 
 #include <cstring>

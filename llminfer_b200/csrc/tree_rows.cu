@@ -6,8 +6,9 @@
 //
 // Layout. 8 warps; a warp owns RT rows, a lane of them the scores of the keys `lane` and lane + 32 and the output channels
 // 4 lane .. + 3. 512 bytes of K or V take four cycles to load from shared memory, the same 16 bytes of Q or P for
-// all lanes one or two, so a warp spans keys and channels and holds several rows. (Half warps of 16 keys with rows of
-// their own: 197 us instead of 171 for 8 nodes of 32 / 8 heads over 32768 keys, 910 instead of 953 for 64.)
+// all lanes one or two, so a warp spans keys and channels and holds several rows: 167 us in a graph for 8 nodes of 32 / 8 heads
+// over 32768 keys, 949 for 64. (Half warps of 16 keys with rows of their own took 197 and 910: slower for few rows, faster
+// for many; one layout was kept, the one of the small trees.)
 // Maximum and P stay inside the warp. Products are packed pairs of FP32 (over channels in S, over output
 // channels in O). K and V tiles come by cp.async, two tiles deep; rows are padded to 132 floats, which
 // spreads 8 of them over all banks. Bound by shared memory and its latency at two warps per scheduler: 64 nodes

@@ -5,8 +5,9 @@
 // c_0 = 0, c_{k+1} = c_k + S_k and S_k the sum of max(p - c_k q, 0) over the vocabulary: one scalar replaces the
 // chain, and a rejection costs one pass over the rows p and q of that node. Accepted nodes cost no row
 // at all, only p and q at the child's token, which are fetched for every node of the tree before
-// the walk starts. Tests and sums are FP64: p, q and u are FP32 or BF16 values, so u q is exact and the
-// outcome does not depend on how the sum was cut.
+// the walk starts. Tests and sums are FP64: p, q and u are FP32 or BF16 values, so u q is exact. S, c and the running
+// sums round in FP64 in an order that follows the cluster's size (so the batch, the vocabulary and the SM count): a test or a
+// threshold within about 2^-50 of equality may fall either way with another size.
 //
 // Without draft probabilities the residual is p without the rejected tokens. One pass per node then
 // serves all its children: R = the sum of p without any child's token; after j rejections the
@@ -19,7 +20,7 @@
 // passes u S, the kept sums of its rounds the round of 32 vectors, and one warp looks through that. A pass is bound by the latency of its loads: a lane
 // has eight vectors of each row in flight (two: 4.4 us a pass over 16000 elements per CTA). Measured: 16 sequences of 32
 // nodes over 128000 words 21 us (up to four passes that depend on one another, about 3 us each, with 2 us of exchange and
-// walk), 64 sequences over 151643 words without draft probabilities 20 us, one of 8 nodes over 32768 words 7 us.
+// walk), 64 sequences over 151643 words without draft probabilities 20 us, one of 8 nodes over 32000 words 7 us.
 #include <cuda_bf16.h>
 
 #include <cstring>
@@ -641,7 +642,7 @@ extern "C" int gqa_tree_verify(const gqa_tree_verify_params* p) {
     a.target_seq = p->target_seq_stride != 0 ? p->target_seq_stride : a.target_node * p->tokens;
     a.draft_seq = p->draft_seq_stride != 0 ? p->draft_seq_stride : a.draft_node * p->tokens;
     if (a.target_node < 0 || a.draft_node < 0 || a.target_seq < 0 || a.draft_seq < 0) return GQA_ERR_SHAPE;
-    // As many CTAs per sequence as leave every lane two vectors of a row and run all at once (one per
+    // As many CTAs per sequence as leave a lane more than one vector of a row and run all at once (one per
     // SM), at most 8 (portable clusters).
     int32_t sms = 0;
     if (current_sm_count(&sms) != GQA_OK) return GQA_ERR_CUDA;

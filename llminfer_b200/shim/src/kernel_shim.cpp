@@ -88,7 +88,9 @@ void mha_kernel_cu(const tensor::Tensor& query, const tensor::Tensor& key_cache,
     p.stream = stream;
     // In the reference's decode step the kernels ahead of attention (QKV GEMV, QK-Norm + RoPE)
     // write the cache row of `pos` only (code/source/model/qwen3_fused.cpp:517-533), so older
-    // rows may be fetched while they finish.
+    // rows may be fetched while they finish. A program that also runs the operators of a tree-drafted step
+    // (gqa_rope_append, gqa_tree_commit), which write more than that row, synchronises the stream between those
+    // and this call.
     p.early_prefetch = 1;
     require_ok(gqa_decode(&p), "gqa_decode");
 }
