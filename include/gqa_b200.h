@@ -692,7 +692,7 @@ int gqa_rope_frequencies(int32_t rotary_dim, double base, int32_t scaling, doubl
  *   q, q_out         [batch, tokens, num_q_heads, 128], *_token_stride elements between tokens (0:
  *                    packed; sequences follow at tokens * stride). q_out may be q with the same stride; else
  *                    no row of it reaches into a row of q (GQA_ERR_UNSUPPORTED).
- *   k_new, v_new     [batch, tokens, num_kv_heads, 128] likewise. They must not overlap the caches.
+ *   k_new, v_new     [batch, tokens, num_kv_heads, 128] likewise. They must not overlap the caches or q_out.
  *   rotary_dim       a multiple of 8, 8 .. 128.
  * All row pointers and strides are 16-byte aligned.
  */
