@@ -116,3 +116,38 @@ def test_commit_of_one_layer_in_a_buffer_of_odd_size(gqa, dtype):
     gqa.tree_commit(k, v, num_kv_heads=2, layout=layout, seq_lens_dev=ints([20]), path=ints([[0, 2, -1, -1]]), kept=ints([2]),
                     seq_lens_out=new)
     assert int(new) == 18 and torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_a_block_other_than_the_first(gqa, dtype):
+    """Without a block table the caches may be any block of a larger one: the same bits as in a cache of its own,
+    and the other blocks stay as they are."""
+    gen = torch.Generator().manual_seed(7)
+    hq, hkv, tokens, cap, vocab = 8, 2, 6, 200, 30
+    parents = PARENTS[:1]
+    freq, _ = gqa.rope_frequencies(64)
+    freq = freq.to(DEV)
+    caches = [torch.randn(3, cap, hkv, D, generator=gen).to(dtype).to(DEV) for _ in range(2)]
+    before = [c.clone() for c in caches]
+    q, kn, vn = (torch.randn(1, tokens, h, D, generator=gen).to(dtype).to(DEV) for h in (hq, hkv, hkv))
+    target = torch.softmax(torch.randn(1, tokens, vocab, generator=gen), -1).to(DEV)
+    words = torch.randint(0, vocab, (1, tokens), generator=gen).int().to(DEV)
+    u = torch.full((1, tokens), 1e-6, device=DEV)  # nearly every draft is taken
+    results = []
+    for block in (0, 2):
+        k, v = caches if block else [c[2].clone() for c in caches]
+        tree = gqa.DraftTree(1, tokens, hq, hkv, DEV, dtype)
+        tree.plan(parents, None, torch.tensor([150]))
+        kw = dict(layout=gqa.layout_reference(3 if block else 1, cap, hkv), fixed_block=block)
+        rot, out = torch.zeros_like(q), torch.zeros_like(q)
+        tree.append(q, kn, vn, k, v, freq=freq, q_out=rot, **kw)
+        tree.attend(rot, k, v, out, **kw)
+        tree.verify(target, None, words, u, torch.full((1,), 0.5, device=DEV))
+        tree.commit(k, v, **kw)
+        assert int(tree.status) == 0 and int(tree.kept) > 1
+        results.append([rot, out, tree.path, tree.next_token, tree.history] + [(c[2] if block else c) for c in (k, v)])
+    assert out.abs().sum() > 0
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    for c, c0 in zip(caches, before):
+        assert torch.equal(c[:2], c0[:2]) and not torch.equal(c[2], c0[2])
